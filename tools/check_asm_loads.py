@@ -10,7 +10,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 src = os.path.join(ROOT, "efficientvlm_amd", "csrc", "attention_mfma.hip")
 with tempfile.TemporaryDirectory() as td:
     out = os.path.join(td, "a.s")
-    subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-S", "--cuda-device-only", "-o", out, src,
+    subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950",
+                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only", "-o", out, src,
                     "-I" + os.path.join(ROOT, "include")], check=True, stderr=subprocess.DEVNULL)
     txt = open(out).read()
 
