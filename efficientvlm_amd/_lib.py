@@ -68,6 +68,16 @@ class XAttnFusedArgs(C.Structure):
                 ("head_gate", _vp), ("scale", _f), ("O", _vp), ("P", _vp)]
 
 
+class PackedAttnArgs(C.Structure):
+    _fields_ = [("dtype", _i), ("Tq", _i), ("Tk", _i), ("S", _i), ("H", _i), ("Hkv", _i), ("dh", _i), ("causal", _i),
+                ("scale", _f), ("Q", _vp), ("K", _vp), ("V", _vp),
+                ("q_tok", _i64), ("q_head", _i64), ("k_tok", _i64), ("k_head", _i64), ("v_tok", _i64), ("v_head", _i64),
+                ("cu_q", _vp), ("cu_k", _vp), ("k_lens", _vp), ("O", _vp), ("O_lo", _vp), ("lse", _vp), ("workspace", _vp),
+                ("dO", _vp), ("dQ", _vp), ("dK", _vp), ("dV", _vp),
+                ("do_tok", _i64), ("do_head", _i64), ("dq_tok", _i64), ("dq_head", _i64), ("dk_tok", _i64), ("dk_head", _i64),
+                ("dv_tok", _i64), ("dv_head", _i64), ("delta", _vp)]
+
+
 # name -> argtypes (every symbol include/evlm_hip.h declares; tests check the library exports all of them)
 SIGNATURES = {
     "evlm_gemm": [C.POINTER(GemmArgs), _vp],
@@ -85,6 +95,9 @@ SIGNATURES = {
     "evlm_attention_bwd": [C.POINTER(AttnBwdArgs), _vp],
     "evlm_attention_lse_supported": [_i, _i, _i, _f],
     "evlm_xattn_fused_fwd": [C.POINTER(XAttnFusedArgs), _vp],
+    "evlm_packed_attention_fwd": [C.POINTER(PackedAttnArgs), _vp],
+    "evlm_packed_attention_bwd": [C.POINTER(PackedAttnArgs), _vp],
+    "evlm_packed_attention_splits": [C.POINTER(PackedAttnArgs)],
     "evlm_mse_fwd": [_i, _vp, _i, _vp, _i64, _f, _vp, _vp],
     "evlm_mse_bwd": [_i, _vp, _i, _vp, _i64, _f, _vp, _vp, _vp],
     "evlm_ce_fwd": [_i, _vp, _i, _i, _i, _vp, _i, _f, _vp, _vp, _vp, _vp],
@@ -98,6 +111,9 @@ SIGNATURES = {
     "evlm_kl_bwd": [_i, _vp, _i, _i, _vp, _i, _i, _i, _f, _f, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "evlm_kl_fwd_rows": [_i, _vp, _i, _i, _vp, _i, _i, _i, _f, _f, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
     "evlm_kl_bwd_rows": [_i, _vp, _i, _i, _vp, _i, _i, _i, _f, _f, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _vp],
+    "evlm_top_logits": [_i, _vp, _i, _i, _i64, _i, _f, _vp, _vp, _vp, _vp],
+    "evlm_kl_top_fwd": [_i, _vp, _i, _i, _i64, _vp, _vp, _vp, _i, _f, _f, _vp, _vp, _vp, _vp, _vp],
+    "evlm_kl_top_bwd": [_i, _vp, _i, _i, _i64, _vp, _vp, _i, _i, _f, _f, _vp, _vp, _vp, _vp, _i64, _i, _vp],
     "evlm_log_softmax_fwd": [_i, _vp, _i, _i, _i, _vp, _i, _vp],
     "evlm_log_softmax_bwd": [_i, _vp, _vp, _i, _i, _i, _vp, _vp],
     "evlm_bert_embed_fwd": [_i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp],

@@ -1,0 +1,456 @@
+// Distillation from a teacher's TOP logits for gfx950: the k largest logits of every row with their classes and the row's
+// log-sum-exp (what a teacher that ran ahead, or offline, keeps of a row of tens of thousands of classes), the loss against
+// a student's whole rows and its gradient.  f32 and bf16 logits, everything else f32.
+//
+//   y = student logits / T,  q = softmax(y) over all C classes,  z_j = kept teacher logits / T of the classes i_j
+//   without the teacher's lse:  p = softmax(z) over the kept classes,        L_r = sum_j p_j (log p_j - log q_{i_j})
+//   with it:  p_j = exp(z_j - lse_t),  p_rest = 1 - sum_j p_j,               L_r += p_rest (log p_rest - log q_rest),
+//             q_rest = the student's mass on the classes that are not kept (one class more for both)
+//   loss = sum_r w_r L_r / R
+//   d L_r / d y_c = M q_c - sum_{j: i_j = c} p_j            kept classes       (M = sum_j p_j + p_rest, 1 up to rounding)
+//                 = q_c / q_rest (M q_rest - p_rest)         all others, with a rest;  M q_c without
+//   An entry whose class lies outside [0, C) takes no part; a row without entries adds nothing and has a zero gradient.
+//
+// All three kernels stream rows: one workgroup per row, 16-byte loads (rows need not be 16-byte aligned: the hardware takes
+// any alignment), sums in f32 in a fixed order.
+#include "common.h"
+
+#define TOP_MAX_K 256
+
+// 8 consecutive elements of a row from any element-aligned address
+template <typename T> __device__ __forceinline__ void load8_any(const T* p, float v[8]);
+template <> __device__ __forceinline__ void load8_any<bf16>(const bf16* p, float v[8]) {
+  bf16x8 t;
+  __builtin_memcpy(&t, p, 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+}
+template <> __device__ __forceinline__ void load8_any<float>(const float* p, float v[8]) {
+  f32x4 t[2];
+  __builtin_memcpy(t, p, 32);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = t[i >> 2][i & 3];
+}
+// elements 8c .. 8c + 7 of a row of C; `fill` behind its end
+template <typename T> __device__ __forceinline__ void row8(const T* x, int c, int C, float fill, float v[8]) {
+  if (8 * c + 8 <= C) { load8_any<T>(x + 8 * (int64_t)c, v); return; }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < C ? to_f(x[8 * (int64_t)c + e]) : fill;
+}
+
+// ---------------------------------------------------------------------------------------------
+// the k largest logits of a row
+// ---------------------------------------------------------------------------------------------
+// order-preserving key of a float: NaN above everything, -0 = +0; 0 is below every value
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0xFFFFFFFFu;
+  const uint32_t u = __float_as_uint(f + 0.0f);
+  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return k == 0xFFFFFFFFu ? __builtin_nanf("") : __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ int block_count(int v, int* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[w] = v;
+  __syncthreads();
+  int t = 0;
+  for (int i = 0; i < nw; ++i) t += red[i];
+  return t;
+}
+
+// One sweep finds every thread's own maximum; the k-th largest of those maxima (its upper 16 bits: a bisection by one wave) is
+// a lower bound of the k-th largest element, and barely more than k elements reach it.  Those are collected and ranked by
+// counting, (value, lower class first) making every element distinct - the result does not depend on the order of collection.
+// Rows with long ties at the bound (more candidates than the list holds) get the exact bound by bisection over the row, first
+// of the value, then of the class among equals.
+#define TOP_NT 512
+#define TOP_CAP 1024
+template <typename T, int NCH>
+__global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict__ logits, int C, int64_t ld, int k, float inv_t,
+                                                            float* __restrict__ values, int32_t* __restrict__ classes,
+                                                            float* __restrict__ lse) {
+  __shared__ float red[16];
+  __shared__ int ired[16];
+  __shared__ uint32_t tops[TOP_NT];
+  __shared__ unsigned long long list[TOP_CAP];
+  __shared__ uint32_t bound;
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t r = blockIdx.x;
+  const T* x = logits + r * ld;
+  const int chunks = (C + 7) >> 3;
+  // rows of up to NCH * 8 * TOP_NT elements stay in registers between the sweeps (NCH = 0: longer ones are read again)
+  float keep[NCH > 0 ? NCH : 1][8];
+  if constexpr (NCH > 0) {
+#pragma unroll
+    for (int n = 0; n < NCH; ++n) {
+      const int c = tid + n * TOP_NT;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) keep[n][e] = -INFINITY;
+      if (c < chunks) row8<T>(x, c, C, -INFINITY, keep[n]);
+    }
+  }
+  auto sweep = [&](auto f) {
+    if constexpr (NCH > 0) {
+#pragma unroll
+      for (int n = 0; n < NCH; ++n) {
+        const int c = tid + n * TOP_NT;
+        if (c < chunks) f(keep[n], 8 * c);
+      }
+    } else {
+      for (int c = tid; c < chunks; c += TOP_NT) {
+        float v[8];
+        row8<T>(x, c, C, -INFINITY, v);
+        f(v, 8 * c);
+      }
+    }
+  };
+  float mx = -INFINITY;
+  bool nan = false, any = false;
+  sweep([&](const float (&v)[8], int) {
+    any = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { mx = fmaxf(mx, v[e]); nan |= v[e] != v[e]; }
+  });
+  tops[tid] = any ? (nan ? 0xFFFFFFFFu : order_key(mx)) : 0u;
+  if (tid == 0) count = 0;
+  const float M = block_max(mx, red);                        // (ends the hand-over of tops and count, too)
+  if (tid < 64) {
+    uint32_t t[TOP_NT / 64], b = 0;
+#pragma unroll
+    for (int j = 0; j < TOP_NT / 64; ++j) t[j] = tops[lane + 64 * j];
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t cand = b | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < TOP_NT / 64; ++j) n += __popcll(__ballot(t[j] >= cand));
+      if (n >= k) b = cand;
+    }
+    if (lane == 0) bound = b;
+  }
+  float s = 0.f;
+  const float top = M * inv_t;
+  if (top != -INFINITY && top != INFINITY)
+    sweep([&](const float (&v)[8], int) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += __expf(fmaf(v[e], inv_t, -top));
+    });
+  const bool bad = block_count(nan ? 1 : 0, ired) != 0;
+  s = block_sum(s, red);
+  if (tid == 0) lse[r] = bad ? __builtin_nanf("") : ((top == -INFINITY || top == INFINITY) ? top : top + __logf(s));
+  const uint32_t b = bound;
+  sweep([&](const float (&v)[8], int i0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t key = order_key(v[e]);
+      if (key >= b && i0 + e < C) {
+        const int at = atomicAdd(&count, 1);
+        if (at < TOP_CAP) list[at] = ((unsigned long long)key << 32) | (uint32_t)~(i0 + e);
+      }
+    }
+  });
+  __syncthreads();
+  int n = count;
+  if (n > TOP_CAP) {                                         // (block-uniform)
+    auto reach = [&](uint32_t lo) {                          // elements with a key >= lo
+      int m = 0;
+      sweep([&](const float (&v)[8], int i0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m += (order_key(v[e]) >= lo && i0 + e < C) ? 1 : 0;
+      });
+      return block_count(m, ired);
+    };
+    uint32_t v0 = 0;                                         // largest key that at least k elements reach
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = v0 | (1u << bit);
+      if (reach(cand) >= k) v0 = cand;
+    }
+    const int more = v0 == 0xFFFFFFFFu ? 0 : reach(v0 + 1), need = k - more;      // `need` of the elements equal to v0
+    int lo = 0, hi = C;                                      // smallest hi with need equal elements below it
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      int m = 0;
+      sweep([&](const float (&v)[8], int i0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m += (order_key(v[e]) == v0 && i0 + e < mid && i0 + e < C) ? 1 : 0;
+      });
+      if (block_count(m, ired) >= need) hi = mid; else lo = mid + 1;
+    }
+    __syncthreads();
+    if (tid == 0) count = 0;
+    __syncthreads();
+    sweep([&](const float (&v)[8], int i0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t key = order_key(v[e]);
+        if (i0 + e < C && (key > v0 || (key == v0 && i0 + e < hi))) {
+          const int at = atomicAdd(&count, 1);
+          if (at < TOP_CAP) list[at] = ((unsigned long long)key << 32) | (uint32_t)~(i0 + e);
+        }
+      }
+    });
+    __syncthreads();
+    n = min(count, TOP_CAP);
+  }
+  for (int i = tid; i < n; i += TOP_NT) {
+    const unsigned long long mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > mine ? 1 : 0;
+    if (rank < k) {
+      values[r * k + rank] = key_value((uint32_t)(mine >> 32));
+      classes[r * k + rank] = (int32_t)~(uint32_t)mine;
+    }
+  }
+}
+
+extern "C" int evlm_top_logits(int dtype, const void* logits, int R, int C, int64_t ld, int k, float inv_t, float* values,
+                               int32_t* classes, float* lse, void* stream_) {
+  hipStream_t stream = (hipStream_t)stream_;
+  EVLM_REQUIRE(logits && values && classes && lse && R > 0 && C > 0 && ld >= C, "evlm_top_logits: bad args");
+  EVLM_REQUIRE(k > 0 && k <= TOP_MAX_K && k <= C, "evlm_top_logits: k = %d is not in 1 .. min(%d, classes)", k, TOP_MAX_K);
+  EVLM_REQUIRE(C <= (1 << 30), "evlm_top_logits: too many classes");
+  EVLM_REQUIRE(inv_t > 0.f && inv_t < 1e30f, "evlm_top_logits: the temperature must be positive and finite");
+  EVLM_DISPATCH_DTYPE(dtype, "evlm_top_logits",
+    if (C <= 8 * 8 * TOP_NT)
+      hipLaunchKernelGGL((top_logits_kernel<T, 8>), dim3(R), dim3(TOP_NT), 0, stream, (const T*)logits, C, ld, k, inv_t, values, classes, lse);
+    else
+      hipLaunchKernelGGL((top_logits_kernel<T, 0>), dim3(R), dim3(TOP_NT), 0, stream, (const T*)logits, C, ld, k, inv_t, values, classes, lse);)
+  EVLM_LAUNCH_CHECK("evlm_top_logits");
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------
+// the loss
+// ---------------------------------------------------------------------------------------------
+#define KDT_NT 512
+// stats of a row, kept for the backward pass
+enum { ST_MAX = 0, ST_SUM, ST_NORM, ST_MASS, ST_MAX_REST, ST_SUM_REST, ST_P_REST, ST_N };
+
+__device__ __forceinline__ double block_sum_f64(double v, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[w] = v;
+  __syncthreads();
+  double t = 0.0;
+  for (int i = 0; i < nw; ++i) t += red[i];
+  return t;
+}
+__device__ __forceinline__ float exp_from(float x, float m) { return m == -INFINITY ? 0.f : __expf(x - m); }   // exp(x - m), x <= m
+
+template <typename T, bool REST>
+__global__ __launch_bounds__(KDT_NT) void kd_top_fwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
+                                                            const int32_t* __restrict__ classes, const float* __restrict__ lse_t,
+                                                            int k, float inv_t, const float* __restrict__ roww,
+                                                            float* __restrict__ stats, float* __restrict__ rowloss) {
+  extern __shared__ uint32_t kept[];                         // REST: one bit per class
+  __shared__ float red[16];
+  __shared__ double dred[16];
+  __shared__ int cls[TOP_MAX_K];
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x;
+  float* st = stats + r * ST_N;
+  const float w = roww ? roww[r] : 1.0f;
+  if (w == 0.f) {                                            // (block-uniform) a row of weight 0 takes no part, whatever it holds
+    if (tid == 0) rowloss[r] = 0.f;
+    return;
+  }
+  const T* x = s + r * ld;
+  const int words = (C + 31) >> 5, chunks = (C + 7) >> 3;
+  if constexpr (REST) {
+    for (int i = tid; i < words; i += KDT_NT) kept[i] = 0u;
+    __syncthreads();
+  }
+  // kept entries: thread j < k holds entry j
+  int ci = -1;
+  float z = -INFINITY, y = -INFINITY;
+  if (tid < k) {
+    ci = classes[r * k + tid];
+    if (ci < 0 || ci >= C) ci = -1;
+    cls[tid] = ci;
+    if (ci >= 0) {
+      z = values[r * k + tid] * inv_t;
+      y = to_f(x[ci]) * inv_t;
+      if constexpr (REST) atomicOr(&kept[ci >> 5], 1u << (ci & 31));
+    }
+  }
+  __syncthreads();
+  // one sweep: running maximum and sum of the row (REST: of the classes that are not kept)
+  float m = -INFINITY, sum = 0.f;
+  for (int c = tid; c < chunks; c += KDT_NT) {
+    float v[8];
+    row8<T>(x, c, C, -INFINITY, v);
+    if constexpr (REST) {
+      const uint32_t bits = (kept[c >> 2] >> (8 * (c & 3))) & 0xFFu;
+      if (bits) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (bits >> e) & 1u ? -INFINITY : v[e];
+      }
+    }
+    float mx = v[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, v[e]);
+    mx *= inv_t;
+    if (mx > m) { sum *= exp_from(m, mx); m = mx; }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += __expf(fmaf(v[e], inv_t, -base));
+  }
+  // (maximum, log of the sum relative to it): one number would lose the sum next to a maximum of the type's lowest value
+  const float m_sweep = block_max(m, red);
+  sum = block_sum(m == -INFINITY ? sum : sum * exp_from(m, m_sweep), red);    // (NaN where the row holds one, even if m is -inf)
+  float top = m_sweep, total = sum;
+  if constexpr (REST) {                                      // + the kept classes, each once
+    bool first = ci >= 0;
+    for (int j = 0; j < tid && j < k; ++j) first = first && cls[j] != ci;
+    top = block_max(fmaxf(first ? y : -INFINITY, m_sweep), red);
+    total = block_sum(first && top != -INFINITY ? expf(y - top) : 0.f, red) + sum * exp_from(m_sweep, top);
+  }
+  const float ls = logf(total), ls_sweep = logf(sum);
+  // teacher.  p_rest is what is left of 1, so p and its sum are formed in 64 bits: one of a few per thousand would keep half of
+  // its digits in 32
+  const float zm = block_max(z, red);
+  float norm, p_rest = 0.f, p = 0.f, mass;
+  if constexpr (REST) {
+    norm = lse_t[r];
+    const double pd = ci >= 0 && z != -INFINITY ? exp((double)z - (double)norm) : 0.0;
+    p = (float)pd;
+    const double kept_mass = block_sum_f64(pd, dred);
+    mass = (float)kept_mass;
+    p_rest = sum == 0.f ? 0.f : (float)fmax(0.0, 1.0 - kept_mass);              // (sum == 0: no class is left for the rest)
+    if (kept_mass != kept_mass) p_rest = mass;
+  } else {
+    const float zs = block_sum(ci >= 0 && z != -INFINITY ? expf(z - zm) : 0.f, red);
+    norm = zm == -INFINITY ? -INFINITY : zm + logf(zs);
+    p = ci >= 0 && z != -INFINITY ? expf(z - zm) / zs : 0.f;
+    mass = zm == -INFINITY ? 0.f : 1.0f;
+    if (zs != zs) mass = zs;
+  }
+  float L = p == 0.f ? 0.f : p * ((z - norm) - ((y - top) - ls));
+  L = block_sum(L, red);
+  if (tid == 0) {
+    if (REST && p_rest != 0.f) L += p_rest * (logf(p_rest) - ((m_sweep - top) + (ls_sweep - ls)));
+    rowloss[r] = w * L;
+    st[ST_MAX] = top; st[ST_SUM] = total; st[ST_NORM] = norm; st[ST_MASS] = mass + p_rest;
+    if constexpr (REST) { st[ST_MAX_REST] = m_sweep; st[ST_SUM_REST] = sum; st[ST_P_REST] = p_rest; }
+  }
+}
+__global__ __launch_bounds__(256) void kd_top_sum_kernel(const float* __restrict__ rowloss, int R, float coef, float* __restrict__ loss) {
+  __shared__ float red[16];
+  float s = 0.f;
+  for (int r = threadIdx.x; r < R; r += 256) s += rowloss[r];
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) loss[0] = s * coef;
+}
+
+// Gradient: one sweep writes every class as if none were kept, then the kept ones are written from their own formula (each
+// duplicate of a class computes the same number).  The barrier between the two orders the stores of one workgroup.
+template <typename T, bool REST>
+__global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
+                                                            const int32_t* __restrict__ classes, int k, float inv_t, float coef,
+                                                            const float* __restrict__ roww, const float* __restrict__ stats,
+                                                            const float* __restrict__ gout, T* __restrict__ ds, int64_t ldd, int acc) {
+  __shared__ int cls[TOP_MAX_K];
+  __shared__ float prob[TOP_MAX_K];
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x;
+  T* d = ds + r * ldd;
+  const float w = roww ? roww[r] : 1.0f;
+  const float* st = stats + r * ST_N;
+  const int dchunks = (int)(ldd >> 3);                       // (ldd % 8 == 0, rows 16-byte aligned)
+  if (w == 0.f || (!REST && st[ST_NORM] == -INFINITY)) {     // (block-uniform) takes no part / no entries
+    if (!acc) {
+      const float zero[8] = {};
+      for (int c = tid; c < dchunks; c += KDT_NT) store8<T>(d + 8 * (int64_t)c, zero);
+    }
+    return;
+  }
+  const float g = gout[0] * coef * w * inv_t;
+  const float top = st[ST_MAX], total = st[ST_SUM], mass = st[ST_MASS], norm = st[ST_NORM];
+  const T* x = s + r * ld;
+  int ci = -1;
+  float y = 0.f, before = 0.f;
+  if (tid < k) {
+    ci = classes[r * k + tid];
+    if (ci < 0 || ci >= C) ci = -1;
+    const float z = ci >= 0 ? values[r * k + tid] * inv_t : -INFINITY;
+    cls[tid] = ci;
+    prob[tid] = z == -INFINITY ? 0.f : expf(z - norm);
+    if (ci >= 0) {
+      y = to_f(x[ci]) * inv_t;
+      if (acc) before = to_f(d[ci]);
+    }
+  }
+  __syncthreads();
+  float mine = 0.f;
+  if (ci >= 0) {
+    float p = 0.f;
+    for (int j = 0; j < k; ++j) p += cls[j] == ci ? prob[j] : 0.f;
+    mine = g * (mass * (expf(y - top) / total) - p) + before;
+  }
+  // the others: f * exp(y - max)
+  const float ref = REST ? st[ST_MAX_REST] : top, ref_sum = REST ? st[ST_SUM_REST] : total;
+  const float share = REST ? mass * (exp_from(ref, top) * ref_sum / total) - st[ST_P_REST] : mass;
+  const float f = ref_sum == 0.f && REST ? 0.f : g * share / ref_sum;           // (no class is left: nothing is written that stays)
+  const float base = ref == -INFINITY && REST ? 0.f : ref;
+  for (int c = tid; c < dchunks; c += KDT_NT) {
+    float v[8];
+    row8<T>(x, c, C, -INFINITY, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < C ? f * __expf(fmaf(v[e], inv_t, -base)) : 0.f;
+    if (acc) {
+      float o[8];
+      load8<T>(d + 8 * (int64_t)c, o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += o[e];
+    }
+    store8<T>(d + 8 * (int64_t)c, v);
+  }
+  __syncthreads();
+  if (ci >= 0) d[ci] = from_f<T>(mine);
+}
+
+static int kd_top_check(const char* name, int R, int C, int64_t ld, int k, float inv_t) {
+  EVLM_REQUIRE(R > 0 && C > 0 && ld >= C, "%s: bad sizes", name);
+  EVLM_REQUIRE(k > 0 && k <= TOP_MAX_K, "%s: k = %d is not in 1 .. %d", name, k, TOP_MAX_K);
+  EVLM_REQUIRE(C <= (1 << 18), "%s: more than 2^18 classes", name);      // (one bit of LDS each: 32 KB)
+  EVLM_REQUIRE(inv_t > 0.f && inv_t < 1e30f, "%s: the temperature must be positive and finite", name);
+  return 0;
+}
+extern "C" int evlm_kl_top_fwd(int dtype, const void* s, int R, int C, int64_t ld, const float* values, const int32_t* classes,
+                               const float* lse_t, int k, float inv_t, float weight, const float* row_weight, float* stats,
+                               float* rowloss, float* loss, void* stream_) {
+  hipStream_t stream = (hipStream_t)stream_;
+  if (int rc = kd_top_check("evlm_kl_top_fwd", R, C, ld, k, inv_t)) return rc;
+  EVLM_REQUIRE(s && values && classes && stats && rowloss && loss, "evlm_kl_top_fwd: null tensor");
+  EVLM_DISPATCH_DTYPE(dtype, "evlm_kl_top_fwd",
+    if (lse_t)
+      hipLaunchKernelGGL((kd_top_fwd_kernel<T, true>), dim3(R), dim3(KDT_NT), (size_t)((C + 31) / 32) * 4, stream, (const T*)s, C, ld, values, classes, lse_t, k, inv_t, row_weight, stats, rowloss);
+    else
+      hipLaunchKernelGGL((kd_top_fwd_kernel<T, false>), dim3(R), dim3(KDT_NT), 0, stream, (const T*)s, C, ld, values, classes, lse_t, k, inv_t, row_weight, stats, rowloss);)
+  EVLM_LAUNCH_CHECK("evlm_kl_top_fwd");
+  hipLaunchKernelGGL(kd_top_sum_kernel, dim3(1), dim3(256), 0, stream, (const float*)rowloss, R, weight / (float)R, loss);
+  EVLM_LAUNCH_CHECK("evlm_kl_top_fwd");
+  return 0;
+}
+extern "C" int evlm_kl_top_bwd(int dtype, const void* s, int R, int C, int64_t ld, const float* values, const int32_t* classes,
+                               int rest, int k, float inv_t, float weight, const float* row_weight, const float* stats,
+                               const float* gout, void* ds, int64_t ldd, int accumulate, void* stream_) {
+  hipStream_t stream = (hipStream_t)stream_;
+  if (int rc = kd_top_check("evlm_kl_top_bwd", R, C, ld, k, inv_t)) return rc;
+  EVLM_REQUIRE(s && values && classes && stats && gout && ds, "evlm_kl_top_bwd: null tensor");
+  EVLM_REQUIRE(ldd >= C && ldd % 8 == 0 && ((uintptr_t)ds & 15) == 0, "evlm_kl_top_bwd: gradient rows must be whole aligned 16-byte pieces");
+  const float coef = weight / (float)R;
+  EVLM_DISPATCH_DTYPE(dtype, "evlm_kl_top_bwd",
+    if (rest)
+      hipLaunchKernelGGL((kd_top_bwd_kernel<T, true>), dim3(R), dim3(KDT_NT), 0, stream, (const T*)s, C, ld, values, classes, k, inv_t, coef, row_weight, stats, gout, (T*)ds, ldd, accumulate);
+    else
+      hipLaunchKernelGGL((kd_top_bwd_kernel<T, false>), dim3(R), dim3(KDT_NT), 0, stream, (const T*)s, C, ld, values, classes, k, inv_t, coef, row_weight, stats, gout, (T*)ds, ldd, accumulate);)
+  EVLM_LAUNCH_CHECK("evlm_kl_top_bwd");
+  return 0;
+}

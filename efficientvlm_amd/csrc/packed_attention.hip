@@ -1,0 +1,817 @@
+// Attention over packed sequences for gfx950: the queries of many sequences laid end to end, their keys likewise (or in the
+// slots of a cache), heads in groups that share a key head, forward and backward, f32 and bf16.
+//
+//   row = one (query token, head).  Query i of a sequence with n queries and m keys sees the keys  j < vis(i),
+//   vis(i) = m  or, causal,  m - n + i + 1  (the last query sees every key: a prompt, a chunk behind a cache and a single
+//   new token are the same formula).
+//   s_j = scale q.k_j,  p_j = 2^(s_j log2e - lse),  lse = log2 sum_j 2^(s_j log2e),  O = sum_j p_j v_j
+//   dP_j = dO.v_j,  delta = dO.O = sum_j p_j dP_j,  dS_j = p_j (dP_j - delta)
+//   dQ = scale sum_j dS_j k_j,   dK_j = scale sum_rows dS_j q,   dV_j = sum_rows p_j dO   (rows of every head of the group)
+//   A row that sees no key has O = 0 and adds nothing to any gradient.
+//
+// All four products of a step are built from two wave-level forms over 32 x 32 blocks:
+//   row_mm   C[r][c] = sum_d tile[r][d] col[c][d]     tile rows from LDS, columns held in registers for the whole loop
+//   col_mm   acc[d][c] += sum_r tile[r][d] P[r][c]    the C of the first product IS the B operand of the second one (the
+//            k-slots of both operands are assigned alike, so P never moves between lanes); bf16 tiles are read by columns
+//            with the transposing LDS reads, f32 tiles with plain ones
+// Forward and dQ hold 32 rows of Q (and dO) as columns and stream keys; dK / dV hold 32 keys as columns and stream rows.
+// A softmax row then lies in two lanes: the running maximum costs one shuffle per block, the sum one at the end.
+//
+// Rows are packed: the gp heads of a group (the largest divisor of the group <= 32) of consecutive tokens fill a block of
+// 32 rows, so one pass over the keys serves all heads that share them - also for a single token.
+//
+// A sequence's blocks are found on the device (find_tile): nothing about the lengths is known to the host, no copy back,
+// and lengths may change between replays of a captured launch.  Every length and start is clamped to the tensors, so no
+// content of cu_q / cu_k / k_lens can make a kernel leave them.  Everything is summed in a fixed order in f32: no atomics.
+#include "common.h"
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+#define PK_LOG2E 1.44269504088896341f
+
+struct PkArgs {
+  const void *Q, *K, *V, *O, *dO;
+  void *out, *out_lo, *dQ, *dK, *dV;
+  const int32_t *cu_q, *cu_k, *k_lens;
+  float *lse, *delta, *part, *part_ml;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head, dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
+  int Tq, Tk, S, H, G, dh;          // G = heads per key head
+  int gp, chunks, units;            // heads packed into a row block, chunks of a group, chunks * key heads
+  int per, tiles;                   // tokens (keys) of a block, grid tiles
+  int splits, causal;
+  float scale, c;                   // c = scale * log2e
+};
+
+// ---- 16-byte fragments ----------------------------------------------------------------------
+template <typename T> struct Frag;
+template <> struct Frag<bf16> { typedef bf16x8 type; };
+template <> struct Frag<float> { typedef f32x4 type; };
+
+__device__ __forceinline__ f32x16 mma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const f32x4& a, const f32x4& b, f32x16 c) {      // 8 of the k-dimension: 4 products of 2
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// Row-major LDS tile [rows][D], 16-byte pieces of a row permuted so that neither the row reads (16 rows, one piece each) nor
+// the column reads (4 rows, a pair of pieces each) meet in a bank: pairs move by the low row bits, the pieces of a pair by bit 3.
+template <typename T, int D> struct Tile {
+  typedef typename Frag<T>::type frag;
+  static constexpr int RB = D * (int)sizeof(T), NC = RB / 16, NS = RB / 32, EP = 16 / (int)sizeof(T);
+  static __device__ __forceinline__ int at(int row, int c) {
+    const int x = NC == 8 ? ((((row >> 1) & 3) << 1) | ((row >> 3) & 1)) : (((row & 7) << 1) | ((row >> 3) & 1));
+    return row * RB + (c ^ x) * 16;
+  }
+  // 32 rows as columns of a product: lane -> row lane & 31, pieces 2s + (lane >> 5); null row: zeros
+  static __device__ __forceinline__ void load_cols(const T* row, int dh, int hh, frag (&f)[NS]) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int e = (2 * s + hh) * EP;
+      frag z = {};
+      f[s] = (row && e < dh) ? *reinterpret_cast<const frag*>(row + e) : z;
+    }
+  }
+  static __device__ __forceinline__ f32x16 row_mm(const char* tile, int r0, const frag (&b)[NS], int lane) {
+    f32x16 acc = {};
+    const int row = r0 + (lane & 31), hh = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) acc = mma(*reinterpret_cast<const frag*>(tile + at(row, 2 * s + hh)), b[s], acc);
+    return acc;
+  }
+  static __device__ __forceinline__ void col_mm(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane);
+};
+
+// bf16: register i of C holds tile row 8 (i >> 2) + 4 (lane >> 5) + (i & 3); registers 8kk .. 8kk + 7 are the B operand of k-step
+// kk, and the A operand takes its 8 rows in that order: two transposing reads of 4 rows x 16 columns each
+template <int D> __device__ __forceinline__ void col_mm_bf16(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+  const int hh = lane >> 5, w = lane & 15, sub = (lane >> 4) & 1;
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    bf16x8 b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = (bf16)p[8 * kk + j];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      const int c = dt * 4 + sub * 2 + ((w & 3) >> 1);
+      bf16x8 a;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = r0 + 16 * kk + 8 * half + 4 * hh + (w >> 2);
+        const bf16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+            (bf16x4 __attribute__((address_space(3)))*)(tile + Tile<bf16, D>::at(row, c) + (w & 1) * 8));
+        a[4 * half + 0] = t[0]; a[4 * half + 1] = t[1]; a[4 * half + 2] = t[2]; a[4 * half + 3] = t[3];
+      }
+      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[dt], 0, 0, 0);
+    }
+  }
+}
+template <int D> __device__ __forceinline__ void col_mm_f32(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+  const int hh = lane >> 5, w = lane & 31;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = r0 + 8 * (i >> 2) + 4 * hh + (i & 3);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      const int e = dt * 32 + w;
+      const float v = *reinterpret_cast<const float*>(tile + Tile<float, D>::at(row, e >> 2) + (e & 3) * 4);
+      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[i], acc[dt], 0, 0, 0);
+    }
+  }
+}
+template <typename T, int D> __device__ __forceinline__ void Tile<T, D>::col_mm(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+  if constexpr (sizeof(T) == 2) col_mm_bf16<D>(tile, r0, p, acc, lane);
+  else col_mm_f32<D>(tile, r0, p, acc, lane);
+}
+// C register -> row of the 32-row block
+__device__ __forceinline__ int c_row(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
+
+// ---- sequences ------------------------------------------------------------------------------
+struct Seq { int qs, qlen, ks, klen; };
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+__device__ __forceinline__ Seq load_seq(const PkArgs& a, int s) {
+  Seq q;
+  q.qs = clampi(a.cu_q[s], 0, a.Tq);
+  q.qlen = clampi(a.cu_q[s + 1], q.qs, a.Tq) - q.qs;
+  q.ks = clampi(a.cu_k[s], 0, a.Tk);
+  q.klen = clampi(a.cu_k[s + 1], q.ks, a.Tk) - q.ks;
+  if (a.k_lens) q.klen = clampi(a.k_lens[s], 0, q.klen);
+  return q;
+}
+__device__ __forceinline__ int vis_of(const PkArgs& a, const Seq& q, int tok) {
+  return a.causal ? clampi(q.klen - q.qlen + tok + 1, 0, q.klen) : q.klen;
+}
+// Block t of all sequences' blocks in order (KEYS: of their keys): the sequence it belongs to and its index there.  Every wave
+// counts 64 sequences at a time.  False: t lies behind the last block (t - total in `over`), the block has nothing to do but the rows
+// outside all sequences.
+template <bool KEYS> __device__ __forceinline__ bool find_tile(const PkArgs& a, int t, Seq& q, int& i, int& over, int& total) {
+  const int lane = threadIdx.x & 63;
+  int64_t before = 0;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    int n = 0;
+    if (s0 + lane < a.S) {
+      const Seq x = load_seq(a, s0 + lane);
+      n = ((KEYS ? x.klen : x.qlen) + a.per - 1) / a.per;
+    }
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    const unsigned long long hit = __ballot(before + incl > t);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      const int64_t first = before + __shfl(incl - n, l, 64);
+      q = load_seq(a, s0 + l);
+      i = (int)(t - first);
+      return true;
+    }
+    before += __shfl(incl, 63, 64);
+  }
+  over = (int)(t - before);
+  total = (int)before;
+  return false;
+}
+// rows outside all sequences ([0, first start), [last end, T)): zeros.  `per_row(row)` by every wave of the surplus blocks
+template <typename F> __device__ __forceinline__ void outside_rows(const int32_t* cu, int S, int T, int index, int count, F per_row) {
+  const int head = S > 0 ? clampi(cu[0], 0, T) : T, tail = S > 0 ? clampi(cu[S], 0, T) : T;
+  const int wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int n = head + (T - tail);
+  for (int64_t r = (int64_t)index * nw + wave; r < n; r += (int64_t)count * nw) per_row(r < head ? (int)r : tail + (int)(r - head));
+}
+
+// ---- staging: `ROWS` rows of a [token][head][dh] tensor -> LDS tile, in two halves (load into registers, store into LDS) ----
+template <typename T, int D, int ROWS, int NT> struct Stage {
+  typedef Tile<T, D> TL;
+  static constexpr int N = ROWS * TL::NC / NT;
+  static_assert(ROWS * TL::NC % NT == 0, "whole pieces per thread");
+  typename TL::frag v[N];
+  // rows first .. first + ROWS - 1 of `base` (row stride `stride` elements); rows >= n repeat row n - 1 (their scores are masked)
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int first, int n, int dh, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int id = tid + k * NT, row = min(first + id / TL::NC, n - 1), e = (id % TL::NC) * TL::EP;
+      typename TL::frag z = {};
+      v[k] = e < dh ? *reinterpret_cast<const typename TL::frag*>(base + row * stride + e) : z;
+    }
+  }
+  // packed rows: row r = (token first + r / gp, head r % gp), zeros behind the last token and in unused rows
+  __device__ __forceinline__ void load_rows(const T* base, int64_t tok_stride, int64_t head_stride, int first, int qlen, int gp,
+                                            int rows_used, int dh, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int id = tid + k * NT, r = id / TL::NC, e = (id % TL::NC) * TL::EP, tok = first + r / gp, h = r % gp;
+      typename TL::frag z = {};
+      v[k] = (e < dh && r < rows_used && tok < qlen)
+                 ? *reinterpret_cast<const typename TL::frag*>(base + tok * tok_stride + h * head_stride + e) : z;
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int id = tid + k * NT;
+      *reinterpret_cast<typename TL::frag*>(tile + TL::at(id / TL::NC, id % TL::NC)) = v[k];
+    }
+  }
+};
+
+// one block of NB * 32 keys for 32 rows: scores, running maximum, probabilities, context.  m is kept as a raw score; it follows
+// the true maximum only when that has grown by more than 2^8 (p then stays <= 2^8, far from any overflow of the f32 sums, and
+// bf16 keeps the same relative precision), so the rescaling of the context is rare.  p is rounded to bf16 for the second
+// product (its sum is not): half a step of 2^-8 relative to each p.
+template <typename T, int D, int NB>
+__device__ __forceinline__ void attend(const char* Ks, const char* Vs, int kt0, int vis, bool mask,
+                                       const typename Frag<T>::type (&qf)[Tile<T, D>::NS], float c, float& m, float& l,
+                                       f32x16 (&o)[D / 32], int lane) {
+  const int hh = lane >> 5;
+  f32x16 s[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) s[b] = Tile<T, D>::row_mm(Ks, 32 * b, qf, lane);
+  if (mask) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = kt0 + 32 * b + c_row(i, hh) < vis ? s[b][i] : -INFINITY;
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  const float mn = fmaxf(m, mx);
+  if (__any((mn - m) * c > 8.0f)) {
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+  }
+  const float mc = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -mc));
+      l += s[b][i];
+    }
+    Tile<T, D>::col_mm(Vs, 32 * b, s[b], o, lane);
+  }
+}
+
+// context / gradient of 32 rows held transposed (lane -> row, registers -> head dim), times `mul`
+template <typename T, int D> __device__ __forceinline__ void store_cols(T* row, int dh, const f32x16 (&o)[D / 32], float mul, int hh) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = dt * 32 + 8 * j + 4 * hh;
+      if (d < dh) {
+        const float v[4] = {o[dt][4 * j] * mul, o[dt][4 * j + 1] * mul, o[dt][4 * j + 2] * mul, o[dt][4 * j + 3] * mul};
+        Vec4<T>::store(row + d, v);
+      }
+    }
+}
+// ... and what the rounding to bf16 took from it, in bf16 as well: O = out + out_lo to 2^-17
+template <typename T, int D> __device__ __forceinline__ void store_rest(T* row, int dh, const f32x16 (&o)[D / 32], float mul, int hh) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = dt * 32 + 8 * j + 4 * hh;
+      if (d < dh) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { const float x = mul_rn(o[dt][4 * j + e], mul); v[e] = x - to_f(from_f<T>(x)); }
+        Vec4<T>::store(row + d, v);
+      }
+    }
+}
+template <typename T> __device__ __forceinline__ void zero_row(T* row, int dh) {
+  for (int d = threadIdx.x & 63; d < dh; d += 64) row[d] = from_f<T>(0.f);
+}
+
+// the surplus blocks of a launch over query blocks: rows outside all sequences are zero
+template <typename T> __device__ __forceinline__ void fwd_outside(const PkArgs& a, int h0, int over, int total) {
+  outside_rows(a.cu_q, a.S, a.Tq, over, a.tiles - total, [&](int r) {
+    for (int h = h0; h < h0 + a.gp; ++h) {
+      zero_row<T>((T*)a.out + ((int64_t)r * a.H + h) * a.dh, a.dh);
+      if (a.lse && (threadIdx.x & 63) == 0) a.lse[(int64_t)h * a.Tq + r] = INFINITY;
+    }
+  });
+}
+
+// ---------------------------------------------------------------------------------------------
+// forward, rows split over the waves: NW * 32 rows of one (sequence, chunk of heads), keys in shared blocks of BN
+// ---------------------------------------------------------------------------------------------
+template <typename T, int D, int NW, int BN>
+__global__ __launch_bounds__(64 * NW, 2) void pk_fwd_rows_kernel(PkArgs a) {
+  typedef Tile<T, D> TL;
+  __shared__ __attribute__((aligned(16))) char sm[2 * BN * TL::RB];
+  char *Ks = sm, *Vs = sm + BN * TL::RB;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
+  Seq q; int ti, over, total;
+  if (!find_tile<false>(a, blockIdx.x / a.units, q, ti, over, total)) { fwd_outside<T>(a, h0, over, total); return; }
+  const int r = wave * 32 + (lane & 31), tok0 = ti * a.per, tok = tok0 + r / a.gp, h = h0 + r % a.gp;
+  const bool valid = r < a.per * a.gp && tok < q.qlen;
+  const int vis = valid ? vis_of(a, q, tok) : 0;
+  const int last = min(tok0 + a.per, q.qlen) - 1;
+  const int nk = vis_of(a, q, last);                                                    // keys any row of the block sees
+  const int w_min = vis_of(a, q, min(tok0 + wave * 32 / a.gp, last)), w_max = vis_of(a, q, min(tok0 + (wave * 32 + 31) / a.gp, last));
+  const bool w_any = tok0 + wave * 32 / a.gp <= last;
+  typename TL::frag qf[TL::NS];
+  TL::load_cols(valid ? (const T*)a.Q + (q.qs + tok) * a.q_tok + h * a.q_head : nullptr, a.dh, hh, qf);
+  const T* Kb = (const T*)a.K + q.ks * a.k_tok + kh * a.k_head;
+  const T* Vb = (const T*)a.V + q.ks * a.v_tok + kh * a.v_head;
+  float m = -INFINITY, l = 0.f;
+  f32x16 o[D / 32] = {};
+  Stage<T, D, BN, 64 * NW> ks, vs;
+  if (nk > 0) { ks.load(Kb, a.k_tok, 0, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, 0, q.klen, a.dh, tid); }
+  for (int kt = 0; kt < nk; kt += BN) {
+    __syncthreads();
+    ks.store(Ks, tid); vs.store(Vs, tid);
+    __syncthreads();
+    if (kt + BN < nk) { ks.load(Kb, a.k_tok, kt + BN, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, kt + BN, q.klen, a.dh, tid); }
+    if (w_any && kt < w_max) attend<T, D, BN / 32>(Ks, Vs, kt, vis, kt + BN > w_min, qf, a.c, m, l, o, lane);
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!valid) return;
+  const int64_t t = q.qs + tok;
+  const float inv = vis > 0 ? 1.0f / l : 0.f;
+  store_cols<T, D>((T*)a.out + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
+  if (sizeof(T) == 2 && a.out_lo) store_rest<T, D>((T*)a.out_lo + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
+  if (a.lse && hh == 0) a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(m, a.c, __builtin_amdgcn_logf(l)) : INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------
+// forward, keys split over the waves (and over `splits` blocks): 32 rows of one (sequence, chunk of heads) - single tokens and very
+// short sequences, where there are too few rows to fill a block of waves but perhaps many keys.  Every wave walks its own
+// 32-key blocks through its own LDS tile (no barrier in the loop) and the waves' sums are joined at the end.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
+  typedef Tile<T, D> TL;
+  constexpr int WB = 2 * 32 * TL::RB > 32 * D * 4 ? 2 * 32 * TL::RB : 32 * D * 4;       // one wave's tiles, later its context
+  __shared__ __attribute__((aligned(16))) char sm[NW * WB];
+  __shared__ float sml[NW][2][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
+  const int rest = blockIdx.x / a.units, split = rest % a.splits;
+  Seq q; int ti, over, total;
+  if (!find_tile<false>(a, rest / a.splits, q, ti, over, total)) {
+    if (split == 0 && a.splits == 1) fwd_outside<T>(a, h0, over, total);
+    return;
+  }
+  const int r = lane & 31, tok0 = ti * a.per, tok = tok0 + r / a.gp, h = h0 + r % a.gp;
+  const bool valid = r < a.per * a.gp && tok < q.qlen;
+  const int vis = valid ? vis_of(a, q, tok) : 0;
+  const int last = min(tok0 + a.per, q.qlen) - 1;
+  const int nk = vis_of(a, q, last), w_min = vis_of(a, q, tok0);
+  // this block's share of the keys: whole 32-key blocks, evenly
+  const int nb = (nk + 31) / 32, b0 = (int)((int64_t)nb * split / a.splits), b1 = (int)((int64_t)nb * (split + 1) / a.splits);
+  char* Ks = sm + wave * WB;
+  char* Vs = Ks + 32 * TL::RB;
+  typename TL::frag qf[TL::NS];
+  TL::load_cols(valid ? (const T*)a.Q + (q.qs + tok) * a.q_tok + h * a.q_head : nullptr, a.dh, hh, qf);
+  const T* Kb = (const T*)a.K + q.ks * a.k_tok + kh * a.k_head;
+  const T* Vb = (const T*)a.V + q.ks * a.v_tok + kh * a.v_head;
+  float m = -INFINITY, l = 0.f;
+  f32x16 o[D / 32] = {};
+  Stage<T, D, 32, 64> ks, vs;
+  int kb = b0 + wave;
+  if (kb < b1) { ks.load(Kb, a.k_tok, kb * 32, q.klen, a.dh, lane); vs.load(Vb, a.v_tok, kb * 32, q.klen, a.dh, lane); }
+  for (; kb < b1; kb += NW) {
+    wave_lds_fence();
+    ks.store(Ks, lane); vs.store(Vs, lane);
+    wave_lds_fence();
+    if (kb + NW < b1) {
+      ks.load(Kb, a.k_tok, (kb + NW) * 32, q.klen, a.dh, lane);
+      vs.load(Vb, a.v_tok, (kb + NW) * 32, q.klen, a.dh, lane);
+    }
+    attend<T, D, 1>(Ks, Vs, kb * 32, vis, kb * 32 + 32 > w_min, qf, a.c, m, l, o, lane);
+  }
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (NW > 1) {
+    // join the waves: wave w sums the row block's columns d = w * D / NW .. of every wave, rescaled to the common maximum
+    wave_lds_fence();
+    float* mine = (float*)(sm + wave * WB);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine[(dt * 32 + c_row(i, hh)) * 32 + r] = o[dt][i];
+    if (hh == 0) { sml[wave][0][r] = m; sml[wave][1][r] = l; }
+    __syncthreads();
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w][0][r]);
+    float L = 0.f, f[NW];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float mw = sml[w][0][r];
+      f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - M) * a.c);
+      L += sml[w][1][r] * f[w];
+    }
+    m = M; l = L;
+    if (!valid) return;
+    const int64_t t = q.qs + tok;
+    const float inv = vis > 0 ? 1.0f / L : 0.f;
+    // thread -> (row r, 4 consecutive d): the 2 NW half-waves take them in turn
+    for (int d = (wave * 2 + hh) * 4; d < a.dh; d += NW * 8) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(((float*)(sm + w * WB))[(d + j) * 32 + r], f[w], v[j]);
+      if (a.splits > 1) {
+        Vec4<float>::store(a.part + (((int64_t)split * a.H + h) * a.Tq + t) * a.dh + d, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= inv;
+        Vec4<T>::store((T*)a.out + (t * a.H + h) * a.dh + d, v);
+        if (sizeof(T) == 2 && a.out_lo) {
+          float lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) lo[j] = v[j] - to_f(from_f<T>(v[j]));
+          Vec4<T>::store((T*)a.out_lo + (t * a.H + h) * a.dh + d, lo);
+        }
+      }
+    }
+    if (wave == 0 && hh == 0) {
+      if (a.splits > 1) {
+        float* ml = a.part_ml + (((int64_t)split * a.H + h) * a.Tq + t) * 2;
+        ml[0] = m; ml[1] = l;
+      } else if (a.lse) {
+        a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(m, a.c, __builtin_amdgcn_logf(l)) : INFINITY;
+      }
+    }
+  } else {
+    if (!valid) return;
+    const int64_t t = q.qs + tok;
+    const float inv = vis > 0 ? 1.0f / l : 0.f;
+    store_cols<T, D>((T*)a.out + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
+    if (sizeof(T) == 2 && a.out_lo) store_rest<T, D>((T*)a.out_lo + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
+    if (a.lse && hh == 0) a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(m, a.c, __builtin_amdgcn_logf(l)) : INFINITY;
+  }
+}
+
+// join of the key splits: one wave per (token, head); a token outside all sequences has no parts and is zero
+template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.Tq * a.H) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = row / a.H;
+  const int h = (int)(row % a.H);
+  const bool inside = a.S > 0 && t >= a.cu_q[0] && t < a.cu_q[a.S];
+  float M = -INFINITY;
+  if (inside)
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[(((int64_t)s * a.H + h) * a.Tq + t) * 2]);
+  float L = 0.f, v0 = 0.f, v1 = 0.f;
+  if (M != -INFINITY)
+    for (int s = 0; s < a.splits; ++s) {
+      const int64_t at = ((int64_t)s * a.H + h) * a.Tq + t;
+      const float ms = a.part_ml[at * 2];
+      if (ms == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f((ms - M) * a.c);
+      L = fmaf(a.part_ml[at * 2 + 1], f, L);
+      if (lane < a.dh) v0 = fmaf(a.part[at * a.dh + lane], f, v0);
+      if (lane + 64 < a.dh) v1 = fmaf(a.part[at * a.dh + lane + 64], f, v1);
+    }
+  const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+  T* o = (T*)a.out + (t * a.H + h) * a.dh;
+  v0 *= inv; v1 *= inv;
+  if (lane < a.dh) o[lane] = from_f<T>(v0);
+  if (lane + 64 < a.dh) o[lane + 64] = from_f<T>(v1);
+  if (sizeof(T) == 2 && a.out_lo) {
+    T* lo = (T*)a.out_lo + (t * a.H + h) * a.dh;
+    if (lane < a.dh) lo[lane] = from_f<T>(v0 - to_f(from_f<T>(v0)));
+    if (lane + 64 < a.dh) lo[lane + 64] = from_f<T>(v1 - to_f(from_f<T>(v1)));
+  }
+  if (a.lse && lane == 0) a.lse[(int64_t)h * a.Tq + t] = M == -INFINITY ? INFINITY : fmaf(M, a.c, __builtin_amdgcn_logf(L));
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward, dQ: NW * 32 rows as in the forward; delta = dO.O of the block's rows is formed here and kept for dK / dV
+// ---------------------------------------------------------------------------------------------
+template <typename T, int D, int NW, int BN>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_kernel(PkArgs a) {
+  typedef Tile<T, D> TL;
+  __shared__ __attribute__((aligned(16))) char sm[2 * BN * TL::RB];
+  char *Ks = sm, *Vs = sm + BN * TL::RB;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
+  Seq q; int ti, over, total;
+  if (!find_tile<false>(a, blockIdx.x / a.units, q, ti, over, total)) {
+    outside_rows(a.cu_q, a.S, a.Tq, over, a.tiles - total, [&](int r) {
+      for (int h = h0; h < h0 + a.gp; ++h) zero_row<T>((T*)a.dQ + r * a.dq_tok + h * a.dq_head, a.dh);
+    });
+    return;
+  }
+  const int r = wave * 32 + (lane & 31), tok0 = ti * a.per, tok = tok0 + r / a.gp, h = h0 + r % a.gp;
+  const bool valid = r < a.per * a.gp && tok < q.qlen;
+  const int vis = valid ? vis_of(a, q, tok) : 0;
+  const int last = min(tok0 + a.per, q.qlen) - 1;
+  const int nk = vis_of(a, q, last);
+  const int w_min = vis_of(a, q, min(tok0 + wave * 32 / a.gp, last)), w_max = vis_of(a, q, min(tok0 + (wave * 32 + 31) / a.gp, last));
+  const bool w_any = tok0 + wave * 32 / a.gp <= last;
+  const int64_t t = q.qs + tok;
+  typename TL::frag qf[TL::NS], df[TL::NS];
+  TL::load_cols(valid ? (const T*)a.Q + t * a.q_tok + h * a.q_head : nullptr, a.dh, hh, qf);
+  TL::load_cols(valid ? (const T*)a.dO + t * a.do_tok + h * a.do_head : nullptr, a.dh, hh, df);
+  float delta = 0.f;
+  {
+    typename TL::frag of[TL::NS];
+    TL::load_cols(valid ? (const T*)a.O + (t * a.H + h) * a.dh : nullptr, a.dh, hh, of);
+#pragma unroll
+    for (int s = 0; s < TL::NS; ++s)
+#pragma unroll
+      for (int j = 0; j < TL::EP; ++j) delta = fmaf((float)df[s][j], (float)of[s][j], delta);
+    if (sizeof(T) == 2) {                                    // O to f32 precision: a rounded O would shift every dS of the row
+      TL::load_cols(valid ? (const T*)a.out_lo + (t * a.H + h) * a.dh : nullptr, a.dh, hh, of);
+#pragma unroll
+      for (int s = 0; s < TL::NS; ++s)
+#pragma unroll
+        for (int j = 0; j < TL::EP; ++j) delta = fmaf((float)df[s][j], (float)of[s][j], delta);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (valid && hh == 0) a.delta[(int64_t)h * a.Tq + t] = delta;
+  }
+  const float lse = valid ? a.lse[(int64_t)h * a.Tq + t] : INFINITY;
+  const T* Kb = (const T*)a.K + q.ks * a.k_tok + kh * a.k_head;
+  const T* Vb = (const T*)a.V + q.ks * a.v_tok + kh * a.v_head;
+  f32x16 acc[D / 32] = {};
+  Stage<T, D, BN, 64 * NW> ks, vs;
+  if (nk > 0) { ks.load(Kb, a.k_tok, 0, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, 0, q.klen, a.dh, tid); }
+  for (int kt = 0; kt < nk; kt += BN) {
+    __syncthreads();
+    ks.store(Ks, tid); vs.store(Vs, tid);
+    __syncthreads();
+    if (kt + BN < nk) { ks.load(Kb, a.k_tok, kt + BN, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, kt + BN, q.klen, a.dh, tid); }
+    if (w_any && kt < w_max) {
+      const bool mask = kt + BN > w_min;
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b) {
+        f32x16 s = TL::row_mm(Ks, 32 * b, qf, lane);
+        const f32x16 dp = TL::row_mm(Vs, 32 * b, df, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse));
+          if (mask) p = kt + 32 * b + c_row(i, hh) < vis ? p : 0.f;
+          s[i] = p * (dp[i] - delta);
+          if (mask) s[i] = kt + 32 * b + c_row(i, hh) < vis ? s[i] : 0.f;
+        }
+        TL::col_mm(Ks, 32 * b, s, acc, lane);
+      }
+    }
+  }
+  if (valid) store_cols<T, D>((T*)a.dQ + t * a.dq_tok + h * a.dq_head, a.dh, acc, a.scale, hh);
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward, dK / dV: NW * 32 keys of one (sequence, key head); the rows of every head of the group stream through LDS
+// ---------------------------------------------------------------------------------------------
+template <typename T, int D, int NW, int BR>
+__global__ __launch_bounds__(64 * NW, 1) void pk_bwd_dkv_kernel(PkArgs a) {
+  typedef Tile<T, D> TL;
+  __shared__ __attribute__((aligned(16))) char sm[2 * BR * TL::RB];
+  __shared__ __attribute__((aligned(16))) float Ls[BR], Ds[BR];
+  __shared__ __attribute__((aligned(16))) int Vis[BR];
+  char *Qs = sm, *Os = sm + BR * TL::RB;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int nkh = a.H / a.G, kh = blockIdx.x % nkh;
+  Seq q; int ti, over, total;
+  if (!find_tile<true>(a, blockIdx.x / nkh, q, ti, over, total)) {
+    outside_rows(a.cu_k, a.S, a.Tk, over, a.tiles - total, [&](int r) {
+      zero_row<T>((T*)a.dK + r * a.dk_tok + kh * a.dk_head, a.dh);
+      zero_row<T>((T*)a.dV + r * a.dv_tok + kh * a.dv_head, a.dh);
+    });
+    return;
+  }
+  const int k0 = ti * a.per, key = k0 + wave * 32 + (lane & 31);
+  const bool valid = key < q.klen;
+  const bool w_any = k0 + wave * 32 < q.klen;
+  typename TL::frag kf[TL::NS], vf[TL::NS];
+  TL::load_cols(valid ? (const T*)a.K + (q.ks + (int64_t)key) * a.k_tok + kh * a.k_head : nullptr, a.dh, hh, kf);
+  TL::load_cols(valid ? (const T*)a.V + (q.ks + (int64_t)key) * a.v_tok + kh * a.v_head : nullptr, a.dh, hh, vf);
+  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+  const int btok = BR / a.gp, used = btok * a.gp;
+  // first query that sees key k0
+  const int first = a.causal ? max(0, k0 - (q.klen - q.qlen)) : 0;
+  Stage<T, D, BR, 64 * NW> qs, os;
+  for (int ch = 0; ch < a.chunks; ++ch) {
+    const int h0 = kh * a.G + ch * a.gp;
+    const T* Qb = (const T*)a.Q + q.qs * a.q_tok + h0 * a.q_head;
+    const T* Ob = (const T*)a.dO + q.qs * a.do_tok + h0 * a.do_head;
+    float lv = INFINITY, dl = 0.f; int vi = 0;
+    auto load = [&](int tok0) {
+      qs.load_rows(Qb, a.q_tok, a.q_head, tok0, q.qlen, a.gp, used, a.dh, tid);
+      os.load_rows(Ob, a.do_tok, a.do_head, tok0, q.qlen, a.gp, used, a.dh, tid);
+      if (tid < BR) {
+        const int tok = tok0 + tid / a.gp;
+        const bool in = tid < used && tok < q.qlen;
+        const int64_t at = (int64_t)(h0 + tid % a.gp) * a.Tq + q.qs + tok;
+        lv = in ? a.lse[at] : INFINITY;
+        dl = in ? a.delta[at] : 0.f;
+        vi = in ? vis_of(a, q, tok) : 0;
+      }
+    };
+    if (first < q.qlen) load(first);
+    for (int tok0 = first; tok0 < q.qlen; tok0 += btok) {
+      __syncthreads();
+      qs.store(Qs, tid); os.store(Os, tid);
+      if (tid < BR) { Ls[tid] = lv; Ds[tid] = dl; Vis[tid] = vi; }
+      __syncthreads();
+      if (tok0 + btok < q.qlen) load(tok0 + btok);
+      // rows see every key of the wave's block unless the block crosses the diagonal or the end
+      const bool mask = (a.causal && vis_of(a, q, tok0) < k0 + wave * 32 + 32) || k0 + wave * 32 + 32 > q.klen;
+      const bool seen = w_any && vis_of(a, q, min(tok0 + btok, q.qlen) - 1) > k0 + wave * 32;
+      if (seen) {
+#pragma unroll
+        for (int b = 0; b < BR / 32; ++b) {
+          f32x16 p = TL::row_mm(Qs, 32 * b, kf, lane);
+          f32x16 ds = TL::row_mm(Os, 32 * b, vf, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r0 = 32 * b + 8 * j + 4 * hh;
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(Ls + r0), d4 = *reinterpret_cast<const f32x4*>(Ds + r0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 4 * j + e;
+              float x = __builtin_amdgcn_exp2f(fmaf(p[i], a.c, -l4[e]));
+              float y = x * (ds[i] - d4[e]);
+              if (mask) {
+                const bool in = valid && key < Vis[r0 + e];
+                x = in ? x : 0.f; y = in ? y : 0.f;
+              }
+              p[i] = x; ds[i] = y;
+            }
+          }
+          TL::col_mm(Os, 32 * b, p, dv, lane);
+          TL::col_mm(Qs, 32 * b, ds, dk, lane);
+        }
+      }
+    }
+  }
+  if (!valid) return;
+  const int64_t kr = q.ks + (int64_t)key;
+  store_cols<T, D>((T*)a.dK + kr * a.dk_tok + kh * a.dk_head, a.dh, dk, a.scale, hh);
+  store_cols<T, D>((T*)a.dV + kr * a.dv_tok + kh * a.dv_head, a.dh, dv, 1.0f, hh);
+}
+
+// ---------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------
+static int largest_divisor(int n, int most) {
+  for (int d = n < most ? n : most; d > 1; --d)
+    if (n % d == 0) return d;
+  return 1;
+}
+static bool pk_few_rows(const evlm_packed_attn_args* x, int gp) {
+  // rows of a sequence and chunk of heads, on average: one wave's worth -> keys are split over the waves instead of rows
+  return (int64_t)x->Tq * gp <= (int64_t)48 * x->S;
+}
+static int pk_splits(const evlm_packed_attn_args* x, int gp) {
+  if (!pk_few_rows(x, gp) || x->Tq == 0 || x->S == 0) return 1;
+  const int64_t blocks = ((int64_t)x->Tq * gp / 32 + x->S) * (x->H / gp);
+  const int64_t keys = x->Tk / x->S;                     // per sequence, on average
+  int64_t n = 512 / (blocks < 1 ? 1 : blocks);
+  if (n > keys / 256) n = keys / 256;
+  return n < 1 ? 1 : (n > 64 ? 64 : (int)n);
+}
+static int pk_check(const evlm_packed_attn_args* x, const char* name) {
+  EVLM_REQUIRE(x->dtype == EVLM_F32 || x->dtype == EVLM_BF16, "%s: bad dtype %d", name, x->dtype);
+  EVLM_REQUIRE(x->Tq >= 0 && x->Tk >= 0 && x->S >= 0 && x->H > 0 && x->Hkv > 0 && x->H % x->Hkv == 0, "%s: bad sizes", name);
+  EVLM_REQUIRE(x->Tq <= (1 << 30) && x->Tk <= (1 << 30) && x->S <= (1 << 30), "%s: more than 2^30 tokens or sequences", name);
+  EVLM_REQUIRE(x->dh > 0 && x->dh <= 128 && x->dh % 8 == 0, "%s: head dim %d is not a multiple of 8 up to 128", name, x->dh);
+  EVLM_REQUIRE(x->scale > 0.f && x->scale < 1e30f, "%s: the scale must be positive and finite", name);
+  EVLM_REQUIRE(x->S == 0 || (x->cu_q && x->cu_k), "%s: no sequence starts", name);
+  const int64_t st[6] = {x->q_tok, x->q_head, x->k_tok, x->k_head, x->v_tok, x->v_head};
+  const int unit = x->dtype == EVLM_BF16 ? 8 : 4;
+  for (int i = 0; i < 6; ++i) EVLM_REQUIRE(st[i] >= 0 && st[i] % unit == 0, "%s: strides must be whole 16-byte pieces", name);
+  EVLM_REQUIRE((((uintptr_t)x->Q | (uintptr_t)x->K | (uintptr_t)x->V) & 15) == 0, "%s: tensors must be 16-byte aligned", name);
+  return 0;
+}
+static PkArgs pk_args(const evlm_packed_attn_args* x) {
+  PkArgs a = {};
+  a.Q = x->Q; a.K = x->K; a.V = x->V; a.out = x->O; a.O = x->O; a.out_lo = x->O_lo; a.lse = x->lse;
+  a.cu_q = x->cu_q; a.cu_k = x->cu_k; a.k_lens = x->k_lens;
+  a.q_tok = x->q_tok; a.q_head = x->q_head; a.k_tok = x->k_tok; a.k_head = x->k_head; a.v_tok = x->v_tok; a.v_head = x->v_head;
+  a.Tq = x->Tq; a.Tk = x->Tk; a.S = x->S; a.H = x->H; a.G = x->H / x->Hkv; a.dh = x->dh;
+  a.gp = largest_divisor(a.G, 32);
+  a.chunks = a.G / a.gp; a.units = a.chunks * x->Hkv;
+  a.causal = x->causal != 0; a.scale = x->scale; a.c = x->scale * PK_LOG2E;
+  a.splits = 1;
+  return a;
+}
+// grid: `units` x (upper bound of the number of blocks + 1, so that there always is a surplus block for the rows outside)
+static int pk_grid(PkArgs& a, int rows, int64_t T, int per, int units, const char* name, unsigned* grid) {
+  a.per = per;
+  const int64_t tiles = T / per + a.S + 1, n = tiles * units * a.splits;
+  if (n > 0x7fffffffll) return evlm_set_error("%s: too many blocks", name);
+  a.tiles = (int)tiles;
+  *grid = (unsigned)n;
+  (void)rows;
+  return 0;
+}
+
+extern "C" int evlm_packed_attention_splits(const evlm_packed_attn_args* x) {
+  if (!x || x->H <= 0 || x->Hkv <= 0 || x->H % x->Hkv) return 1;
+  return pk_splits(x, largest_divisor(x->H / x->Hkv, 32));
+}
+
+template <typename T, int D> static int pk_fwd_launch(PkArgs& a, bool few, hipStream_t stream) {
+  unsigned grid;
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+  if (few) {
+    if (int rc = pk_grid(a, 32, a.Tq, 32 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
+    if (a.splits == 1 && a.S > 0 && a.Tk / a.S <= 64)
+      hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 1>), dim3(grid), dim3(64), 0, stream, a);
+    else
+      hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 4>), dim3(grid), dim3(256), 0, stream, a);
+    if (a.splits > 1) {
+      EVLM_LAUNCH_CHECK("evlm_packed_attention_fwd");
+      const int64_t rows = (int64_t)a.Tq * a.H;
+      hipLaunchKernelGGL((pk_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+    }
+  } else {
+    if (int rc = pk_grid(a, 128, a.Tq, 128 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
+    hipLaunchKernelGGL((pk_fwd_rows_kernel<T, D, 4, BN>), dim3(grid), dim3(256), 0, stream, a);
+  }
+  EVLM_LAUNCH_CHECK("evlm_packed_attention_fwd");
+  return 0;
+}
+
+#define PK_DISPATCH(x, CALL)                                                                                   \
+  ((x)->dtype == EVLM_BF16 ? ((x)->dh <= 64 ? CALL<bf16, 64> : CALL<bf16, 128>)                                \
+                           : ((x)->dh <= 64 ? CALL<float, 64> : CALL<float, 128>))
+
+extern "C" int evlm_packed_attention_fwd(const evlm_packed_attn_args* x, void* stream_) {
+  EVLM_REQUIRE(x, "evlm_packed_attention_fwd: no arguments");
+  if (int rc = pk_check(x, "evlm_packed_attention_fwd")) return rc;
+  if (x->Tq == 0) return 0;
+  EVLM_REQUIRE(x->Q && x->O && (x->Tk == 0 || (x->K && x->V)), "evlm_packed_attention_fwd: null tensor");
+  PkArgs a = pk_args(x);
+  const bool few = x->S > 0 && pk_few_rows(x, a.gp);
+  a.splits = pk_splits(x, a.gp);
+  if (a.splits > 1) {
+    EVLM_REQUIRE(x->workspace, "evlm_packed_attention_fwd: %d key splits need a workspace", a.splits);
+    a.part = (float*)x->workspace;
+    a.part_ml = a.part + (int64_t)a.splits * x->H * x->Tq * x->dh;
+  }
+  return PK_DISPATCH(x, pk_fwd_launch)(a, few, (hipStream_t)stream_);
+}
+
+template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, hipStream_t stream) {
+  unsigned grid;
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+  const char* name = "evlm_packed_attention_bwd";
+  const int nkh = a.H / a.G;
+  if (a.Tq > 0) {
+    if (few) {
+      if (int rc = pk_grid(a, 32, a.Tq, 32 / a.gp, a.units, name, &grid)) return rc;
+      hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 1, 32>), dim3(grid), dim3(64), 0, stream, a);
+    } else {
+      if (int rc = pk_grid(a, 128, a.Tq, 128 / a.gp, a.units, name, &grid)) return rc;
+      hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 4, BN>), dim3(grid), dim3(256), 0, stream, a);
+    }
+    EVLM_LAUNCH_CHECK(name);
+  }
+  if (a.Tk > 0) {
+    if (a.S > 0 && a.Tk / a.S <= 48) {
+      if (int rc = pk_grid(a, 32, a.Tk, 32, nkh, name, &grid)) return rc;
+      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 1, 32>), dim3(grid), dim3(64), 0, stream, a);
+    } else {
+      if (int rc = pk_grid(a, 128, a.Tk, 128, nkh, name, &grid)) return rc;
+      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 4, 32>), dim3(grid), dim3(256), 0, stream, a);
+    }
+    EVLM_LAUNCH_CHECK(name);
+  }
+  return 0;
+}
+
+extern "C" int evlm_packed_attention_bwd(const evlm_packed_attn_args* x, void* stream_) {
+  EVLM_REQUIRE(x, "evlm_packed_attention_bwd: no arguments");
+  const char* name = "evlm_packed_attention_bwd";
+  if (int rc = pk_check(x, name)) return rc;
+  EVLM_REQUIRE(x->Tq == 0 || (x->Q && x->O && x->dO && x->dQ && x->lse && x->delta), "%s: null tensor", name);
+  EVLM_REQUIRE(x->Tq == 0 || x->dtype == EVLM_F32 || x->O_lo, "%s: bf16 needs O_lo", name);
+  EVLM_REQUIRE(x->Tk == 0 || (x->K && x->V && x->dK && x->dV), "%s: null tensor", name);
+  const int64_t st[8] = {x->do_tok, x->do_head, x->dq_tok, x->dq_head, x->dk_tok, x->dk_head, x->dv_tok, x->dv_head};
+  const int unit = x->dtype == EVLM_BF16 ? 8 : 4;
+  for (int i = 0; i < 8; ++i) EVLM_REQUIRE(st[i] >= 0 && st[i] % unit == 0, "%s: strides must be whole 16-byte pieces", name);
+  EVLM_REQUIRE((((uintptr_t)x->dO | (uintptr_t)x->dQ | (uintptr_t)x->dK | (uintptr_t)x->dV) & 15) == 0, "%s: tensors must be 16-byte aligned", name);
+  PkArgs a = pk_args(x);
+  a.dO = x->dO; a.dQ = x->dQ; a.dK = x->dK; a.dV = x->dV; a.delta = x->delta;
+  a.do_tok = x->do_tok; a.do_head = x->do_head; a.dq_tok = x->dq_tok; a.dq_head = x->dq_head;
+  a.dk_tok = x->dk_tok; a.dk_head = x->dk_head; a.dv_tok = x->dv_tok; a.dv_head = x->dv_head;
+  const bool few = x->S > 0 && pk_few_rows(x, a.gp);
+  return PK_DISPATCH(x, pk_bwd_launch)(a, few, (hipStream_t)stream_);
+}

@@ -8,6 +8,7 @@ Compute dtype: activations are either torch.float32 (exact-fp32 parity path, fp3
 torch.bfloat16 (fast path: bf16 storage, fp32 accumulate).  Parameters stay fp32 (checkpoint ABI); the
 bf16 path reads packed bf16 compute copies from `WeightCache`.
 """
+import contextlib
 import ctypes as C
 import os
 import math
@@ -1490,6 +1491,134 @@ def cross_attention(q, kv, H, dh, scale, mask=None, gate=None, want_probs=True, 
                             None, 1.0, None, kv_grad)[:2]
 
 
+# ---------------------------------------------------------------------------------------------------
+# attention over packed sequences (no map, no padding)
+# ---------------------------------------------------------------------------------------------------
+def _on_device_of(t):
+    """launches go to the device the tensors live on, whatever the current one is"""
+    return torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
+
+
+def _heads3(x):
+    """x [tokens, heads, dh] as the packed kernels read it: heads in whole 16-byte pieces, 16-byte aligned (slices of a packed
+    projection are; anything else is copied).  Returns (tensor, token stride, head stride)."""
+    unit = 16 // x.element_size()
+    st = [0 if n <= 1 else s for n, s in zip(x.shape[:2], x.stride()[:2])]
+    if (x.stride(2) != 1 and x.shape[2] > 1) or any(s % unit for s in st) or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        st = [0 if n <= 1 else s for n, s in zip(x.shape[:2], x.stride()[:2])]
+    return x, st[0], st[1]
+
+
+def _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal):
+    """(args, tensors the pointers in them belong to) of one packed-attention launch"""
+    (q, qt, qh), (k, kt, kh), (v, vt, vh) = _heads3(q), _heads3(k), _heads3(v)
+    a = L.PackedAttnArgs(dtype=L.dt(q), Tq=q.shape[0], Tk=k.shape[0], S=cu_q.numel() - 1, H=q.shape[1], Hkv=k.shape[1],
+                         dh=q.shape[2], causal=int(bool(causal)), scale=scale, Q=L.ptr(q), K=L.ptr(k), V=L.ptr(v),
+                         q_tok=qt, q_head=qh, k_tok=kt, k_head=kh, v_tok=vt, v_head=vh,
+                         cu_q=L.ptr(cu_q), cu_k=L.ptr(cu_k), k_lens=L.ptr(k_lens))
+    return a, (q, k, v)
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, k_lens, scale, causal):
+        need = any(ctx.needs_input_grad[:3])
+        with _on_device_of(q):
+            a, keep = _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal)
+            Tq, H, dh = q.shape
+            O = torch.empty((Tq, H, dh), dtype=q.dtype, device=q.device)
+            lse = torch.empty((H, Tq), dtype=torch.float32, device=q.device) if need else None
+            lo = torch.empty_like(O) if need and q.dtype == torch.bfloat16 else None     # (what rounding took from O)
+            splits = _lib().evlm_packed_attention_splits(C.byref(a))
+            ws = torch.empty(splits * H * Tq * (dh + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+            a.O, a.O_lo, a.lse, a.workspace = L.ptr(O), L.ptr(lo), L.ptr(lse), L.ptr(ws)
+            L.check(_lib().evlm_packed_attention_fwd(C.byref(a), L.stream()), "packed_attention_fwd")
+        if need:
+            ctx.save_for_backward(*keep, cu_q, cu_k, k_lens, O, lo, lse)
+            ctx.meta = (scale, causal)
+        return O
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dO):
+        q, k, v, cu_q, cu_k, k_lens, O, lo, lse = ctx.saved_tensors
+        scale, causal = ctx.meta
+        with _on_device_of(q):
+            a, keep = _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal)
+            dO, ot, oh = _heads3(dO)
+            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            # (the kernels write every key of every sequence and the rows outside all of them; unfilled room is left alone)
+            alloc = torch.empty if k_lens is None else torch.zeros
+            dk, dv = alloc(k.shape, dtype=k.dtype, device=k.device), alloc(v.shape, dtype=v.dtype, device=v.device)
+            delta = torch.empty_like(lse)
+            a.O, a.O_lo, a.lse, a.delta, a.dO, a.do_tok, a.do_head = L.ptr(O), L.ptr(lo), L.ptr(lse), L.ptr(delta), L.ptr(dO), ot, oh
+            for name, t in (("dq", dq), ("dk", dk), ("dv", dv)):
+                setattr(a, "dQ" if name == "dq" else ("dK" if name == "dk" else "dV"), L.ptr(t))
+                setattr(a, name + "_tok", t.stride(0))
+                setattr(a, name + "_head", t.stride(1))
+            L.check(_lib().evlm_packed_attention_bwd(C.byref(a), L.stream()), "packed_attention_bwd")
+        return dq, dk, dv, None, None, None, None, None
+
+
+def packed_attention(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=True):
+    """Attention over packed sequences: the queries of S sequences end to end in q [Tq, H, dh], their keys and values in
+    k, v [Tk, Hkv, dh] (H a multiple of Hkv: heads h H/Hkv .. share key head h; slices of a packed q | k | v buffer are
+    read in place).  f32 or bf16, dh a multiple of 8 up to 128.  Returns O [Tq, H, dh].
+
+    cu_q, cu_k: int32 [S + 1] on the GPU, ascending - sequence s owns queries cu_q[s] .. cu_q[s+1]-1 and keys cu_k[s] ..
+    cu_k[s+1]-1 (cu_k None: the same).  k_lens: int32 [S], the filled part of each key range (a cache with room; None: all of
+    it) - what lies behind it is never read.  They are read by the kernels only: no host synchronisation, and a captured
+    launch follows their contents.
+    causal: query i of n sees keys j < m - n + i + 1 of m, so the last query sees every key (a whole prompt, a chunk behind a
+    cache, a single new token).  scale: 1 / sqrt(dh) unless given, positive.
+    A row that sees no key, and a row outside all sequences, is zero; gradients likewise.  Within one sequence, keys that
+    causality hides from a row must hold finite values (their probability is an exact 0, 0 * inf is not).
+
+    The padded kinds are self_attention / cross_attention (with the probability map as an output); the decoder masks of
+    eff_bert.py:975-996 are the causal form here."""
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise RuntimeError(f"packed_attention: {n} must be [tokens, heads, head dim], got {tuple(t.shape)}")
+        if t.dtype != q.dtype:
+            raise TypeError("packed_attention: q, k and v must have one dtype")
+    L.dt(q)
+    H, dh = q.shape[1], q.shape[2]
+    if k.shape != v.shape or k.shape[2] != dh:
+        raise RuntimeError(f"packed_attention: k {tuple(k.shape)} and v {tuple(v.shape)} must agree, with q's head dim {dh}")
+    Hkv = k.shape[1]
+    if H == 0 or Hkv == 0 or H % Hkv:
+        raise RuntimeError(f"packed_attention: {H} query heads are no multiple of {Hkv} key heads")
+    if dh == 0 or dh > 128 or dh % 8:
+        raise RuntimeError(f"packed_attention: head dim {dh} is not a multiple of 8 up to 128")
+    if max(q.shape[0], k.shape[0]) > 1 << 30:
+        raise RuntimeError("packed_attention: more than 2^30 tokens")
+    scale = dh ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise RuntimeError(f"packed_attention: the scale must be positive and finite, got {scale}")
+    if cu_k is None:
+        cu_k = cu_q
+        if k.shape[0] != q.shape[0]:
+            raise RuntimeError("packed_attention: without cu_k there must be as many keys as queries")
+    for n, t in (("cu_q", cu_q), ("cu_k", cu_k), ("k_lens", k_lens)):
+        if t is None:
+            continue
+        if t.dtype != torch.int32 or t.dim() != 1:
+            raise TypeError(f"packed_attention: {n} must be a 1-d int32 tensor")
+    if cu_q.numel() < 1 or cu_k.numel() != cu_q.numel() or (k_lens is not None and k_lens.numel() != cu_q.numel() - 1):
+        raise RuntimeError("packed_attention: cu_q and cu_k need S + 1 entries, k_lens S")
+    _same_device(q, k, v, cu_q, cu_k, k_lens)
+    L.require_cuda(q)
+    return _PackedAttention.apply(q, k, v, cu_q.contiguous(), cu_k.contiguous(),
+                                  None if k_lens is None else k_lens.contiguous(), scale, bool(causal))
+
+
 _PIN_CHUNKS, _PIN_USED = [], 0            # pinned int64 chunks (every one stays alive: pending uploads read them)
 _PIN_CHUNK_WORDS = 1 << 17                # 1 MiB each: ~700 tables of 45 copies
 _DEV_CHUNKS = {}                          # device index -> [int64 device chunk (outside any graph pool), words used]
@@ -2418,6 +2547,125 @@ def soft_cross_entropy(predicts, targets, temperature=1.0, ragged=None):
     """ragged (ops.Ragged): the logits are [rows, tokens, classes] of a bucket-padded batch - rows / tokens beyond the real
     extents take no part (the mean keeps the padded count: the caller rescales)"""
     return _KL.apply(predicts, targets.detach(), 1.0 / float(temperature), ragged)
+
+
+# ---- distillation from a teacher's top logits --------------------------------------------------------
+TOP_MAX_K = 256
+
+
+def _top_rows(x, name):
+    """logits [..., C] as rows with a row stride >= C (rows of any alignment)"""
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise RuntimeError(f"{name}: logits must be [..., classes], got {tuple(x.shape)}")
+    Cn = x.shape[-1]
+    x2 = x.reshape(-1, Cn)
+    if (x2.stride(1) != 1 and Cn > 1) or (x2.shape[0] > 1 and x2.stride(0) < Cn):
+        x2 = x2.contiguous()
+    return x2, x2.shape[0], Cn, x2.stride(0) if x2.shape[0] > 1 else Cn
+
+
+def top_logits(logits, k, temperature=1.0):
+    """what is kept of a teacher's logits [..., C] (f32 / bf16): (values f32 [..., k] descending, classes int32 [..., k],
+    lse f32 [...]) - the k <= 256 largest of each row (equal ones: the lower class first; NaN above everything) and
+    log sum_c exp(logits / temperature) over the whole row.  For soft_cross_entropy_top, in place of the C logits that
+    soft_cross_entropy reads (GeneralDistill.py:84-89).  No gradient."""
+    k, T = int(k), float(temperature)
+    L.dt(logits)
+    x = logits.detach()
+    if x.dim() < 1 or not 1 <= k <= min(TOP_MAX_K, x.shape[-1]):
+        raise RuntimeError(f"top_logits: k = {k} must lie in 1 .. min({TOP_MAX_K}, classes) of {tuple(logits.shape)}")
+    if not 1e-30 < T < 1e30:
+        raise RuntimeError(f"top_logits: the temperature must be positive and finite, got {temperature}")
+    if x.shape[-1] > 1 << 30:
+        raise RuntimeError("top_logits: more than 2^30 classes")
+    L.require_cuda(x)
+    lead = x.shape[:-1]
+    with _on_device_of(x):
+        values = torch.empty((*lead, k), dtype=torch.float32, device=x.device)
+        classes = torch.empty((*lead, k), dtype=torch.int32, device=x.device)
+        lse = torch.empty(lead, dtype=torch.float32, device=x.device)
+        if lse.numel():
+            x2, R, Cn, ld = _top_rows(x, "top_logits")
+            L.check(_lib().evlm_top_logits(L.dt(x2), L.ptr(x2), R, Cn, ld, k, 1.0 / T, L.ptr(values), L.ptr(classes),
+                                           L.ptr(lse), L.stream()), "top_logits")
+    return values, classes, lse
+
+
+class _KLTop(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, s, values, classes, lse, weight, inv_t):
+        with _on_device_of(s):
+            s2, R, Cn, ld = _top_rows(s, "soft_cross_entropy_top")
+            k = values.shape[-1]
+            out = torch.empty((), dtype=torch.float32, device=s.device)
+            work = torch.empty(8 * R, dtype=torch.float32, device=s.device)      # 7 statistics of each row, then the rows' losses
+            rowloss = C.c_void_p(work.data_ptr() + 28 * R)
+            L.check(_lib().evlm_kl_top_fwd(L.dt(s2), L.ptr(s2), R, Cn, ld, L.ptr(values), L.ptr(classes), L.ptr(lse), k, inv_t,
+                                           1.0, L.ptr(weight), L.ptr(work), rowloss, L.ptr(out), L.stream()), "kl_top_fwd")
+        ctx.save_for_backward(s2, values, classes, weight, work)
+        ctx.meta = (R, Cn, ld, k, inv_t, lse is not None, s.shape)
+        ctx.join = getattr(s, "_evlm_join", None)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        s2, values, classes, weight, work = ctx.saved_tensors
+        R, Cn, ld, k, inv_t, rest, shape = ctx.meta
+        with _on_device_of(s2):
+            gc = g.to(torch.float32).contiguous()
+            ldd = _pad8(Cn)
+            acc, join = _join_target(ctx, R, ldd, s2.dtype)
+            ds = acc if acc is not None else torch.empty((R, ldd), dtype=s2.dtype, device=s2.device)   # (padding: zeroed by the kernel)
+            L.check(_lib().evlm_kl_top_bwd(L.dt(s2), L.ptr(s2), R, Cn, ld, L.ptr(values), L.ptr(classes), int(rest), k, inv_t,
+                                           1.0, L.ptr(weight), L.ptr(work), L.ptr(gc), L.ptr(ds), ldd, int(acc is not None),
+                                           L.stream()), "kl_top_bwd")
+        if acc is not None:
+            return None, None, None, None, None, None
+        d = ds[:, :Cn] if ldd != Cn else ds
+        d = d.unflatten(0, shape[:-1]) if len(shape) > 2 else d.view(shape)
+        if join is not None:                   # first joined writer: the join point hands (view, buffer) on
+            join.buf = (d, ds)
+            return None, None, None, None, None, None
+        return d, None, None, None, None, None
+
+
+def soft_cross_entropy_top(predicts, values, classes, lse=None, temperature=1.0, row_weight=None):
+    """soft_cross_entropy against a teacher of which only the top logits are left (top_logits): predicts [..., C] student
+    logits (f32 / bf16, gradient), values f32 and classes int32 / int64 [..., k], k <= 256.  Mean over the rows of
+    row_weight [...] (default 1) times KL(p || softmax(predicts / temperature)), a device scalar:
+      lse None:  p = softmax(values / temperature) over the kept classes (the teacher renormalised);
+      lse [...]: p = exp(values / temperature - lse), lse being the teacher's log-sum-exp at the SAME temperature; the mass that
+                 is not kept counts as one more class, against the student's mass on the classes that are not kept.
+    Entries whose class lies outside 0 .. C-1 take no part (padding of rows that kept fewer; -1 by custom); a row without
+    entries, and a row of weight 0, adds nothing and has a zero gradient, whatever it holds.  A class that stands twice in a row
+    counts as two entries.  Gradients reach `predicts` only; logits aliased by join_grads are served like soft_cross_entropy's."""
+    T = float(temperature)
+    L.dt(predicts)
+    if predicts.dim() < 1 or predicts.numel() == 0:
+        raise RuntimeError(f"soft_cross_entropy_top: no rows in {tuple(predicts.shape)}")
+    lead = predicts.shape[:-1]
+    k = values.shape[-1] if values.dim() else 0
+    if values.shape != (*lead, k) or classes.shape != values.shape or not 1 <= k <= TOP_MAX_K:
+        raise RuntimeError(f"soft_cross_entropy_top: values {tuple(values.shape)} and classes {tuple(classes.shape)} must be "
+                           f"{tuple(lead)} + (k <= {TOP_MAX_K},)")
+    if classes.dtype not in (torch.int32, torch.int64):
+        raise TypeError("soft_cross_entropy_top: classes must be int32 or int64")
+    for n, t in (("values", values), ("lse", lse), ("row_weight", row_weight)):
+        if t is not None and not t.dtype.is_floating_point:
+            raise TypeError(f"soft_cross_entropy_top: {n} must be floating point")
+        if t is not None and n != "values" and t.shape != lead:
+            raise RuntimeError(f"soft_cross_entropy_top: {n} {tuple(t.shape)} must have one entry per row {tuple(lead)}")
+    if not 1e-30 < T < 1e30:
+        raise RuntimeError(f"soft_cross_entropy_top: the temperature must be positive and finite, got {temperature}")
+    if predicts.shape[-1] > 1 << 18:
+        raise RuntimeError("soft_cross_entropy_top: more than 2^18 classes")
+    _same_device(predicts, values, classes, lse, row_weight)
+    L.require_cuda(predicts)
+    if classes.dtype == torch.int64:           # (a class that does not fit stays outside)
+        classes = classes.clamp(-1, predicts.shape[-1]).to(torch.int32)
+    f32 = lambda t: None if t is None else t.detach().to(torch.float32).contiguous()
+    return _KLTop.apply(predicts, f32(values), classes.contiguous(), f32(lse), f32(row_weight), 1.0 / T)
 
 
 class _LogSoftmax(torch.autograd.Function):

@@ -289,6 +289,44 @@ int evlm_copy_grouped(const int64_t* table, int n_units, int total_blocks, void*
 int evlm_copy_few(const void* const* src, void* const* dst, const int64_t* nbytes, int n, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Attention over PACKED sequences: the queries of S sequences laid end to end, their keys likewise (or in the slots of a
+ * cache), H query heads in groups of H / Hkv that share a key head; no probability map, no padding.
+ *   Q [Tq, H, dh], K / V [Tk, Hkv, dh] through their token and head strides (elements; whole 16-byte pieces, so slices of a
+ *   packed q | k | v projection work as they are), 16-byte aligned; dh a multiple of 8 up to 128; O [Tq, H, dh] contiguous.
+ *   Sequence s owns the queries cu_q[s] .. cu_q[s+1]-1 and the keys cu_k[s] .. cu_k[s+1]-1, of which the first k_lens[s] are
+ *   filled (NULL: all).  cu_q, cu_k (int32 [S+1], ascending) and k_lens are DEVICE memory and are read by the kernels: one
+ *   captured launch serves every batch of the same Tq, Tk, S.  Starts and lengths are clamped to the tensors.
+ *   causal: query i of n sees keys j < m - n + i + 1 of m (the last query sees all).  A row that sees no key, and a row outside
+ *   all sequences, has O = 0; so have the gradients of keys that no row sees.
+ *   lse [H, Tq] f32 (forward: written if given; backward: as the forward wrote it).  delta [H, Tq] f32: backward scratch.
+ *   workspace: forward, only if evlm_packed_attention_splits() > 1: that many times H * Tq * (dh + 2) floats (uninitialised).
+ * The decoder side of the reference pads its answers to the longest (eff_bert.py:317-355 over [B, L] rows, the causal mask of
+ * :975-996); packed rows do the same arithmetic without the padding.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  int dtype;
+  int Tq, Tk, S, H, Hkv, dh;
+  int causal;
+  float scale;                  /* > 0 */
+  const void* Q; const void* K; const void* V;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  const int32_t* cu_q; const int32_t* cu_k; const int32_t* k_lens;
+  void* O;
+  void* O_lo;                   /* bf16: O - (O rounded to bf16), [Tq, H, dh]; forward: written if given, backward: needed (delta) */
+  float* lse;
+  void* workspace;
+  /* backward only: dO, dQ, dK, dV through their strides; every element of dQ is written, of dK / dV all but the unfilled
+     parts of slots (k_lens), which are left as they were */
+  const void* dO; void* dQ; void* dK; void* dV;
+  int64_t do_tok, do_head, dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
+  float* delta;
+} evlm_packed_attn_args;
+int evlm_packed_attention_fwd(const evlm_packed_attn_args* a, void* stream);
+int evlm_packed_attention_bwd(const evlm_packed_attn_args* a, void* stream);
+/* number of parts the forward cuts the keys into (a rule on Tq, Tk, S, H, Hkv); 1: no workspace */
+int evlm_packed_attention_splits(const evlm_packed_attn_args* a);
+
+/* ------------------------------------------------------------------------------------------------
  * Fused cross-attention FORWARD: K/V projection of the image tokens + Q K^T + softmax + P V (+ the map) in one launch.
  *   K = X Wk^T + bk, V = X Wv^T + bv  (Wkv: [2d, d] rows Wk then Wv, bias_kv [2d] likewise - the packed layout the
  *   two-launch path uses);  S = scale * Q K^T + mask[bq, k];  P = softmax(S);  O = (P V) * head_gate[h].
@@ -399,6 +437,24 @@ int evlm_kl_bwd_rows(int dtype_s, const void* s, int lds, int dtype_t, const voi
                      float inv_t, float weight, const float* lse_s, const float* lse_t, const float* gout,
                      void* ds, int ldds, int accumulate, const int32_t* ext, int row_inner, int inner_slot, int outer_slot,
                      void* stream);
+
+/* Distillation from a teacher's TOP logits (soft_cross_entropy, GeneralDistill.py:84-89, for a teacher of which only the k
+ * largest logits of a row were kept).
+ * evlm_top_logits: values f32 [R, k] (descending) and classes int32 [R, k] of the k <= 256 largest of C logits (equal ones: lower
+ * class first; NaN above everything), lse f32 [R] = log sum_c exp(logits * inv_t).  Rows have stride ld, of any alignment.
+ * evlm_kl_top_fwd: *loss = weight / R * sum_r row_weight[r] L_r,  L_r = KL(p || softmax(s * inv_t)) with p = softmax(values * inv_t)
+ * over the kept classes (lse_t NULL), or p = exp(values * inv_t - lse_t) with the remaining mass as one more class, against
+ * the student's mass on the classes that are not kept.  Entries with a class outside 0 .. C-1 take no part; rows of weight
+ * 0 (row_weight NULL: all 1) neither.  stats f32 [7 R], rowloss f32 [R]: scratch, stats are read by the backward pass.
+ * evlm_kl_top_bwd: ds [R, ldd] = (accumulate: +=) the gradient, padding columns as zeros; `rest` != 0 where lse_t was given. */
+int evlm_top_logits(int dtype, const void* logits, int R, int C, int64_t ld, int k, float inv_t, float* values,
+                    int32_t* classes, float* lse, void* stream);
+int evlm_kl_top_fwd(int dtype, const void* s, int R, int C, int64_t ld, const float* values, const int32_t* classes,
+                    const float* lse_t, int k, float inv_t, float weight, const float* row_weight, float* stats,
+                    float* rowloss, float* loss, void* stream);
+int evlm_kl_top_bwd(int dtype, const void* s, int R, int C, int64_t ld, const float* values, const int32_t* classes,
+                    int rest, int k, float inv_t, float weight, const float* row_weight, const float* stats,
+                    const float* gout, void* ds, int64_t ldd, int accumulate, void* stream);
 
 /* row-wise log_softmax (for the soft-label ITC branch, xvlm.py:411-414) and its backward */
 int evlm_log_softmax_fwd(int dtype, const void* x, int R, int C, int ld, void* y, int ldy, void* stream);

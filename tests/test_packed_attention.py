@@ -1,0 +1,478 @@
+"""ops.packed_attention against its definition in 64 bits.
+
+Tolerances count roundings (u = half a step of the storage type: 2^-8 bf16, 2^-24 f32) and are per element:
+  probability p_ij        relative error rel_i: the scores' f32 dot products ((dh + 8) 2^-24 scale sum_d |q_d k_d|, twice: for the score
+                          and for the maximum / log-sum-exp), the f32 sums over n keys and the 2^x / division ((n + 16) 2^-24);
+                          rounded once more to the storage type as an operand of the next product (u)
+  O                       u |O| + (u + rel_i) sum_j p |v|
+  delta = dO.O            with the stored O: sum_d |dO| (error of O) + dh 2^-24 sum_d |dO O|            =: e_i
+  dS = p (dP - delta)     u |dS| + rel_i p (|dP| + |delta|) + p (e_i + (dh + 8) 2^-24 sum_d |dO v|)     =: f_ij
+  dQ, dK, dV              u |x| + sum of the operands' errors, + (n + 16) 2^-24 of the absolute sum (n terms summed in f32)
+"""
+import ctypes
+import math
+import os
+import re
+
+import pytest
+import torch
+
+from efficientvlm_amd import ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+BF16, F32 = torch.bfloat16, torch.float32
+F = 2.0 ** -24
+
+
+def starts(lens, first=0):
+    out = [first]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+def definition(q, k, v, dout, q0, lq, k0, lk, causal, scale, u):
+    """(O, dQ, dK, dV) in 64 bits and the bound of each element's error, on the CPU"""
+    q, k, v = (t.detach().double().cpu() for t in (q, k, v))
+    dout = torch.zeros_like(q) if dout is None else dout.detach().double().cpu()
+    H, dh = q.shape[1:]
+    G = H // k.shape[1]
+    val = [torch.zeros_like(t) for t in (q, q, k, v)]
+    tol = [torch.zeros_like(t) for t in (q, q, k, v)]
+    for a, n, b, m in zip(q0, lq, k0, lk):
+        if n == 0 or m == 0:
+            continue
+        seen = torch.ones(n, m, dtype=torch.bool)
+        if causal:
+            seen = torch.arange(m)[None, :] <= torch.arange(n)[:, None] + (m - n)
+        for h in range(H):
+            Q, dO = q[a:a + n, h], dout[a:a + n, h]
+            K, V = k[b:b + m, h // G], v[b:b + m, h // G]
+            S = (Q @ K.T * scale).masked_fill(~seen, -math.inf)
+            P = torch.softmax(S, 1).nan_to_num(0.0)                  # (rows that see nothing)
+            O = P @ V
+            rel = (2 * (dh + 8) * F * scale * (Q.abs() @ K.abs().T)).masked_fill(~seen, 0).amax(1) + (m + 16) * F
+            A = P @ V.abs()
+            eO = u * O.abs() + (u + rel)[:, None] * A
+            dP = dO @ V.T
+            delta = (dO * O).sum(1)
+            dS = P * (dP - delta[:, None])
+            e = (dO.abs() * eO).sum(1) + dh * F * (dO * O).abs().sum(1)
+            f = (u * dS.abs() + rel[:, None] * P * (dP.abs() + delta.abs()[:, None])
+                 + P * (e[:, None] + (dh + 8) * F * (dO.abs() @ V.abs().T)))
+            absS = P * (dP.abs() + delta.abs()[:, None])
+            val[0][a:a + n, h], tol[0][a:a + n, h] = O, eO
+            x = scale * dS @ K
+            val[1][a:a + n, h], tol[1][a:a + n, h] = x, u * x.abs() + scale * ((f + (m + 16) * F * absS) @ K.abs())
+            rows = G * n + 16
+            val[2][b:b + m, h // G] += scale * dS.T @ Q
+            tol[2][b:b + m, h // G] += scale * (f + rows * F * absS).T @ Q.abs()
+            val[3][b:b + m, h // G] += P.T @ dO
+            tol[3][b:b + m, h // G] += ((u + rel[:, None] + rows * F) * P).T @ dO.abs()
+    tol[2] += u * val[2].abs()
+    tol[3] += u * val[3].abs()
+    return val, tol
+
+
+def check(got, val, tol, names=("O", "dQ", "dK", "dV")):
+    for g, x, t, n in zip(got, val, tol, names):
+        g = g.detach().double().cpu()
+        assert g.shape == x.shape
+        over = ((g - x).abs() - t - 1e-30).nan_to_num(math.inf)
+        assert over.max() <= 0, f"{n}: {int((over > 0).sum())} of {over.numel()} elements off, worst by {over.max():.3e} over its bound"
+
+
+def problem(dtype, H, Hkv, dh, lq, lk=None, slots=0, before=0, behind=0, seed=0, layout="plain"):
+    """q, k, v, dout, the starts and lengths; `slots`: room behind every key range, `before` / `behind`: rows outside"""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    same = lk is None
+    lk = list(lq) if same else list(lk)
+    room = [n + slots for n in lk]
+    q0, k0 = starts(lq, before), starts(room, before if same and not slots else 0)
+    nq = q0[-1] + behind
+    nk = nq if same and not slots else k0[-1] + behind
+    if layout == "qkv" and nq == nk:
+        buf = r(nq, H + 2 * Hkv, dh).to(dtype).cuda()
+        q, k, v = buf[:, :H], buf[:, H:H + Hkv], buf[:, H + Hkv:]
+    elif layout == "heads_first":                 # [heads, tokens, dh] storage
+        q, k, v = (r(h, n, dh).to(dtype).cuda().transpose(0, 1) for h, n in ((H, nq), (Hkv, nk), (Hkv, nk)))
+    elif layout == "odd":                         # rows that are no whole 16-byte pieces: copied by the call
+        q, k, v = (r(n, h, dh + 1).to(dtype).cuda()[..., 1:] for h, n in ((H, nq), (Hkv, nk), (Hkv, nk)))
+    else:
+        q, k, v = (r(n, h, dh).to(dtype).cuda() for h, n in ((H, nq), (Hkv, nk), (Hkv, nk)))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    return dict(q=q, k=k, v=v, dout=r(nq, H, dh).to(dtype).cuda(), cu_q=i32(q0), cu_k=i32(k0),
+                k_lens=i32(lk) if slots else None, q0=q0[:-1], lq=list(lq), k0=k0[:-1], lk=lk)
+
+
+def run(p, causal=True, scale=None, backward=True):
+    q, k, v = (p[n].detach().requires_grad_(backward) for n in "qkv")
+    out = ops.packed_attention(q, k, v, p["cu_q"], p["cu_k"], k_lens=p["k_lens"], scale=scale, causal=causal)
+    return (out,) + (torch.autograd.grad(out, (q, k, v), p["dout"]) if backward else ())
+
+
+def both(p, causal=True, scale=None, backward=True):
+    u = 2.0 ** -8 if p["q"].dtype == BF16 else F
+    sc = p["q"].shape[2] ** -0.5 if scale is None else scale
+    val, tol = definition(p["q"], p["k"], p["v"], p["dout"] if backward else None, p["q0"], p["lq"], p["k0"], p["lk"], causal, sc, u)
+    got = run(p, causal, scale, backward)
+    check(got, val, tol)
+    return got, val, tol
+
+
+# ---- refusals (no GPU) ------------------------------------------------------------------------------
+def test_refusals():
+    t = lambda *s, dt=F32: torch.zeros(*s, dtype=dt)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    ok = dict(q=t(4, 4, 16), k=t(4, 2, 16), v=t(4, 2, 16), cu_q=cu)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.packed_attention(**ok)
+    bad = [(dict(q=t(4, 64)), RuntimeError, "tokens, heads"), (dict(k=t(4, 3, 16), v=t(4, 3, 16)), RuntimeError, "multiple"),
+           (dict(v=t(4, 2, 16, dt=BF16)), TypeError, "one dtype"), (dict(v=t(5, 2, 16)), RuntimeError, "agree"),
+           (dict(q=t(4, 4, 24)), RuntimeError, "head dim 24"), (dict(k=t(5, 2, 16), v=t(5, 2, 16)), RuntimeError, "as many keys"),
+           (dict(cu_q=cu.long()), TypeError, "int32"), (dict(cu_k=torch.zeros(3, dtype=torch.int32)), RuntimeError, "entries"),
+           (dict(k_lens=torch.zeros(2, dtype=torch.int32)), RuntimeError, "entries"), (dict(cu_q=cu[:0]), RuntimeError, "entries"),
+           (dict(scale=0.0), RuntimeError, "scale"), (dict(scale=-1.0), RuntimeError, "scale"), (dict(scale=math.nan), RuntimeError, "scale")]
+    for change, err, match in bad:
+        with pytest.raises(err, match=match):
+            ops.packed_attention(**{**ok, **change})
+    for d in (12, 136):
+        with pytest.raises(RuntimeError, match="head dim"):
+            ops.packed_attention(t(4, 4, d), t(4, 2, d), t(4, 2, d), cu)
+    with pytest.raises(TypeError, match="float16"):
+        ops.packed_attention(*(t(4, 2, 16, dt=torch.float16) for _ in range(3)), cu)
+
+
+def test_c_entry_refuses_before_any_launch():
+    """the C entries check what a kernel assumes on the host; nothing reaches a device here"""
+    from efficientvlm_amd import _lib
+    lib = _lib.load()
+    base = dict(dtype=_lib.BF16, Tq=4, Tk=4, S=1, H=4, Hkv=2, dh=64, scale=0.125, Q=4096, K=4096, V=4096, O=4096, cu_q=4096, cu_k=4096,
+                q_tok=256, q_head=64, k_tok=128, k_head=64, v_tok=128, v_head=64)
+    for change in (dict(dtype=7), dict(dh=72 + 4), dict(dh=136), dict(H=5), dict(scale=0.0), dict(Q=4098), dict(k_tok=12), dict(O=None),
+                   dict(cu_q=None), dict(K=None), dict(Tq=-1)):
+        a = _lib.PackedAttnArgs(**{**base, **change})
+        assert lib.evlm_packed_attention_fwd(ctypes.byref(a), None) != 0, change
+        assert lib.evlm_last_error()
+    assert lib.evlm_packed_attention_bwd(ctypes.byref(_lib.PackedAttnArgs(**base)), None) != 0       # no dO, lse, ...
+    assert lib.evlm_packed_attention_fwd(ctypes.byref(_lib.PackedAttnArgs(**{**base, "Tq": 0})), None) == 0
+
+
+def test_struct_layout_matches_header():
+    from efficientvlm_amd import _lib
+    src = open(os.path.join(ROOT, "include", "evlm_hip.h")).read()
+    body = re.search(r"typedef struct \{((?:(?!typedef struct).)*?)\}\s*evlm_packed_attn_args", src, flags=re.S).group(1)
+    fields = []
+    for decl in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
+        names = re.sub(r"^(const\s+)?[A-Za-z_0-9]+\s*\**", "", decl.strip())
+        fields += [n.strip().lstrip("*").strip() for n in re.sub(r"(const\s+)?\bvoid\*|int32_t\*", "", names).split(",") if n.strip()]
+    assert fields == [f[0] for f in _lib.PackedAttnArgs._fields_]
+
+
+# ---- values and gradients ---------------------------------------------------------------------------
+LENGTHS = {
+    "ones": [1] * 9,
+    "answers": [3, 7, 1, 12, 5, 0, 16, 2, 9, 4],
+    "edges": [31, 32, 33, 0, 1, 127, 128, 129, 63, 65],
+    "one_long": [517],
+    "ragged": [200, 3, 90, 1, 333],
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths", sorted(LENGTHS))
+def test_lengths(dtype, causal, lengths):
+    both(problem(dtype, 4, 2, 64, LENGTHS[lengths]), causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads", [(1, 1), (3, 1), (12, 12), (10, 2), (14, 2), (32, 1), (40, 1), (71, 1)])
+def test_head_groups(dtype, heads):
+    both(problem(dtype, heads[0], heads[1], 32, [17, 40, 1, 70], seed=heads[0]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dh", [8, 24, 40, 64, 72, 96, 128])
+def test_head_dims(dtype, dh):
+    both(problem(dtype, 4, 2, dh, [50, 1, 140], seed=dh))
+    both(problem(dtype, 4, 2, dh, [5, 1, 9, 2], seed=dh))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+def test_other_keys_and_rows_that_see_none(dtype, causal):
+    """more keys than queries (a chunk behind a cache), fewer (causal: the first queries see nothing), none at all"""
+    (out, dq, dk, dv), _, _ = both(problem(dtype, 6, 2, 64, [4, 20, 9, 1, 0, 70, 3], [40, 5, 0, 300, 7, 70, 1]), causal)
+    if causal:
+        assert (out[4:4 + 15] == 0).all() and (dq[4:4 + 15] == 0).all()           # 20 queries, 5 keys
+    assert (out[24:33] == 0).all() and (dq[24:33] == 0).all()                     # no keys
+    assert (dk[345:352] == 0).all() and (dv[345:352] == 0).all()                  # no queries
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,dh", [((12, 12), 64), ((32, 8), 128), ((8, 1), 128), ((6, 2), 40)])
+@pytest.mark.parametrize("lk", [[1, 2, 31], [33, 64, 500, 0, 1], [9000, 4097], [20000]])
+def test_single_tokens_behind_caches(dtype, heads, dh, lk):
+    both(problem(dtype, *heads, dh, [1] * len(lk), lk, slots=9), backward=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_few_tokens_behind_caches_train(dtype):
+    both(problem(dtype, 8, 2, 64, [1, 3, 2], [1500, 700, 2100], slots=5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("layout", ["qkv", "heads_first", "odd"])
+def test_layouts(dtype, layout):
+    p = problem(dtype, 4, 2, 64, [40, 9, 150], layout=layout)
+    p["dout"] = p["dout"].transpose(0, 1).contiguous().transpose(0, 1)
+    both(p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lq", [[5, 3], [150, 40]])
+def test_rows_outside_all_sequences(dtype, lq):
+    """rows before the first and behind the last sequence: zero outputs and gradients, whatever they hold"""
+    p = problem(dtype, 4, 2, 64, lq, before=3, behind=37)
+    inside = torch.zeros(p["q"].shape[0], dtype=torch.bool, device="cuda")
+    inside[3:3 + sum(lq)] = True
+    for n in "qkv":
+        p[n][~inside] = math.nan
+    p["dout"][~inside] = math.nan
+    got = run(p)
+    for t in got:
+        assert (t[~inside] == 0).all()
+    q = dict(p)
+    for n in ("q", "k", "v", "dout"):
+        q[n] = p[n].masked_fill(~inside[:, None, None], 0.0)
+    for a, b in zip(got, run(q)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lq,lk", [([1, 1, 1], [40, 3, 2000]), ([60, 5, 130], [70, 5, 333])])
+def test_unfilled_room_and_neighbours_are_not_read(dtype, lq, lk):
+    """NaN behind the filled part of the slots, and NaN in ONE sequence, stay where they are"""
+    p = problem(dtype, 4, 2, 64, lq, lk, slots=11)
+    want = run(p)
+    for b, n in zip(p["k0"], p["lk"]):
+        for t in ("k", "v"):
+            p[t][b + n:b + n + 11] = math.nan
+    got = run(p)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert all((got[i][b + n:b + n + 11] == 0).all() for i in (2, 3) for b, n in zip(p["k0"], p["lk"]))
+    p["v"][p["k0"][1]] = math.nan                                                # a key every row of sequence 1 sees
+    got = run(p)
+    a, n = p["q0"][1], p["lq"][1]
+    assert got[0][a:a + n].isnan().all()
+    keep = torch.ones(got[0].shape[0], dtype=torch.bool, device="cuda")
+    keep[a:a + n] = False
+    assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1][keep], want[1][keep])
+
+
+@pytest.mark.gpu
+def test_scores_far_apart_and_infinite():
+    """scores whose differences pass 2^100, and keys with -inf scores: an exact 0, no NaN"""
+    p = problem(F32, 2, 2, 64, [70], seed=3)
+    p["q"] = p["q"].abs()
+    p["k"] = p["k"] * 40
+    both(p, scale=1.0)
+    p = problem(F32, 2, 1, 64, [1, 40], [50, 90], seed=4)
+    p["q"] = p["q"].abs() + 0.1
+    low = [3, 60, 61]
+    want = {n: p[n].clone() for n in "kv"}
+    for j in low:
+        p["k"][j] = -math.inf
+    got = run(p, causal=False, backward=False)[0]
+    assert got.isfinite().all()
+    S = (p["q"].double().cpu().transpose(0, 1) @ p["k"].double().cpu()[:, 0].T.nan_to_num(neginf=-1e300)) / 8
+    ref = []
+    for i in range(41):
+        b, n = (0, 50) if i == 0 else (50, 90)
+        ref.append(torch.softmax(S[:, i, b:b + n], 1) @ want["v"].double().cpu()[b:b + n, 0])
+    err = (got.double().cpu() - torch.stack(ref)).abs().max()
+    assert err <= 200 * F * want["v"].abs().max().item() * 8             # (n + dh + scores' size) roundings of values up to max |v|
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """directional differences of the definition in 64 bits (step 1e-5: truncation ~ 1e-10) against the f32 kernels' gradients"""
+    p = problem(F32, 4, 2, 32, [30, 1, 45, 7], seed=5)
+    got = run(p)
+    val, tol = definition(p["q"], p["k"], p["v"], p["dout"], p["q0"], p["lq"], p["k0"], p["lk"], True, 32 ** -0.5, F)
+
+    def loss(**move):
+        x = {n: p[n].double() + (1e-5 * move[n] if n in move else 0) for n in "qkv"}
+        o = definition(x["q"], x["k"], x["v"], None, p["q0"], p["lq"], p["k0"], p["lk"], True, 32 ** -0.5, F)[0][0]
+        return (o * p["dout"].double().cpu()).sum()
+    for i, n in enumerate("qkv"):
+        d = torch.randn(p[n].shape, generator=torch.Generator().manual_seed(i), dtype=torch.float64)
+        diff = (loss(**{n: d.cuda()}) - loss(**{n: -d.cuda()})) / 2e-5
+        mine = (got[1 + i].double().cpu() * d).sum()
+        assert abs(mine - diff) <= (tol[1 + i] * d.abs()).sum() + 1e-7 * (1 + abs(diff))
+
+
+# ---- how it is called -------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [[4, 9, 2], [300, 130]])
+def test_same_bits_every_time(lq):
+    p = problem(BF16, 8, 2, 64, lq)
+    first = run(p)
+    for _ in range(3):
+        for a, b in zip(run(p), first):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_only_some_gradients_and_no_grad():
+    p = problem(BF16, 4, 2, 64, [30, 80])
+    want = run(p)
+    k = p["k"].detach().requires_grad_()
+    out = ops.packed_attention(p["q"], k, p["v"], p["cu_q"])
+    assert torch.equal(out, want[0])
+    out.backward(p["dout"])
+    assert torch.equal(k.grad, want[2])
+    with torch.no_grad():
+        out = ops.packed_attention(p["q"], k, p["v"], p["cu_q"])
+    assert not out.requires_grad and torch.equal(out, want[0])
+    with pytest.raises(RuntimeError):                                             # no second derivative, and it says so
+        q = p["q"].float().detach().requires_grad_()
+        g, = torch.autograd.grad(ops.packed_attention(q, p["k"].float(), p["v"].float(), p["cu_q"]).sum(), q, create_graph=True)
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_gradients_of_shared_storage_and_broadcast():
+    """slices of one projection and key heads broadcast from one: autograd sums what the call hands back"""
+    p = problem(F32, 4, 4, 32, [20, 33])
+    one = p["k"][:, :1].contiguous().detach().requires_grad_()
+    out = ops.packed_attention(p["q"], one.expand(-1, 4, -1), p["v"], p["cu_q"])
+    out.backward(p["dout"])
+    full = p["k"][:, :1].expand(-1, 4, -1).contiguous()
+    val, tol = definition(p["q"], full, p["v"], p["dout"], p["q0"], p["lq"], p["k0"], p["lk"], True, 32 ** -0.5, F)
+    check([one.grad], [val[2].sum(1, keepdim=True)], [tol[2].sum(1, keepdim=True) + 8 * F * val[2].abs().sum(1, keepdim=True)], ["dK"])
+    qkv = torch.randn(53, 12, 32, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_()
+    ops.packed_attention(qkv[:, :4], qkv[:, 4:8], qkv[:, 8:], p["cu_q"]).sum().backward()       # (dO: an expanded scalar)
+    val, tol = definition(qkv[:, :4], qkv[:, 4:8], qkv[:, 8:], torch.ones(53, 4, 32), p["q0"], p["lq"], p["k0"], p["lk"], True, 32 ** -0.5, F)
+    check([qkv.grad], [torch.cat(val[1:], 1)], [torch.cat(tol[1:], 1)], ["dQKV"])
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    z = lambda *s: torch.zeros(*s, dtype=BF16, device="cuda")
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    assert ops.packed_attention(z(0, 4, 64), z(0, 2, 64), z(0, 2, 64), i(0)).shape == (0, 4, 64)
+    assert (ops.packed_attention(z(5, 4, 64) + 1, z(5, 2, 64), z(5, 2, 64) + 1, i(0)) == 0).all()             # no sequences
+    assert (ops.packed_attention(z(5, 4, 64) + 1, z(0, 2, 64), z(0, 2, 64), i(0, 5), i(0, 0)) == 0).all()     # no keys
+    q, k, v = (t.requires_grad_() for t in (z(5, 4, 64), z(7, 2, 64), z(7, 2, 64)))
+    out = ops.packed_attention(q, k, v, i(0, 0, 0), i(0, 3, 3))
+    out.sum().backward()
+    assert all((t == 0).all() for t in (out, q.grad, k.grad, v.grad))
+    q, k, v = (t.requires_grad_() for t in (z(0, 4, 64), z(7, 2, 64), z(7, 2, 64)))
+    ops.packed_attention(q, k, v, i(0, 0), i(0, 7)).sum().backward()
+    assert q.grad.shape == (0, 4, 64) and (k.grad == 0).all() and (v.grad == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu_q,cu_k,k_lens", [([0, 99, 20], None, None), ([-5, 30, 12], None, None), ([40, 2, 1], None, None),
+                                              ([0, 10, 20], [0, 1 << 30, -7], None), ([0, 10, 20], [0, 10, 20], [1 << 30, -3]),
+                                              ([2147483647, -2147483648, 2147483647], None, None)])
+def test_starts_that_make_no_sense_stay_inside_the_tensors(cu_q, cu_k, k_lens):
+    """clamped on the device: the values are nobody's business, the accesses are"""
+    i32 = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")
+    guard = torch.zeros(3, 20, 4, 64, dtype=F32, device="cuda")
+    q, k, v = (guard[j].clone().requires_grad_() for j in range(3))
+    out = ops.packed_attention(q, k, v, i32(cu_q), i32(cu_k), k_lens=i32(k_lens))
+    torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    torch.cuda.synchronize()
+    assert out.shape == (20, 4, 64)
+
+
+@pytest.mark.gpu
+def test_many_sequences():
+    """more sequences than one wave counts at a time, empty ones among them"""
+    g = torch.Generator().manual_seed(0)
+    lens = torch.randint(0, 5, (700,), generator=g).tolist()
+    both(problem(BF16, 2, 1, 32, lens))
+    both(problem(F32, 2, 2, 32, lens, [3 * n for n in lens]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk", [([5, 9, 2], None), ([140, 60, 33], None), ([1, 1, 1], [3000, 1200, 2])])
+def test_capture_follows_the_lengths(lq, lk):
+    """one captured forward + backward, replayed on other lengths of the same totals, eager work in between"""
+    p = problem(BF16, 8, 2, 64, lq, lk, slots=3 if lk else 0)
+    q, k, v = (p[n].detach().clone().requires_grad_() for n in "qkv")
+
+    def step():
+        out = ops.packed_attention(q, k, v, p["cu_q"], p["cu_k"], k_lens=p["k_lens"])
+        return (out,) + torch.autograd.grad(out, (q, k, v), p["dout"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    n = sum(lq)
+    for turn, cut in enumerate([lq, [1, n - 2, 1] if lk is None else [1, 1, 1], lq]):
+        p["cu_q"].copy_(torch.tensor(starts(cut), dtype=torch.int32))
+        if lk is None:
+            p["cu_k"].copy_(p["cu_q"])
+        else:
+            p["k_lens"].copy_(torch.tensor([max(1, x - 7 * turn) for x in lk], dtype=torch.int32))
+        with torch.no_grad():
+            q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(turn)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in static]
+        want = run({**p, "q": q, "k": k, "v": v})
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """calls in flight on two streams share nothing"""
+    ps = [problem(BF16, 8, 2, 64, [1, 1], [4000, 2500], slots=1, seed=s) for s in range(2)]
+    want = [run(p) for p in ps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ps]
+    got = [None, None]
+    for _ in range(5):
+        for i, (p, s) in enumerate(zip(ps, streams)):
+            with torch.cuda.stream(s):
+                got[i] = run(p)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_keys_behind_two_to_the_31():
+    """offsets of a long cache: K is 2^31 + elements, the sequence lies behind them"""
+    tokens, Hkv, dh = (1 << 31) // (8 * 128) + 600, 8, 128
+    k = torch.zeros(tokens, Hkv, dh, dtype=BF16, device="cuda")
+    p = problem(BF16, 8, Hkv, dh, [1, 70], [300, 200])
+    k[tokens - 500:] = p["k"]
+    cu_k = torch.tensor([tokens - 500, tokens - 200, tokens], dtype=torch.int32, device="cuda")
+    got = ops.packed_attention(p["q"], k, k, p["cu_q"], cu_k)
+    want = ops.packed_attention(p["q"], p["k"], p["k"], p["cu_q"], p["cu_k"])
+    # (the split of the keys over blocks follows the tensors' sizes: equal values, not equal bits)
+    val, tol = definition(p["q"], p["k"], p["k"], None, p["q0"], p["lq"], p["k0"], p["lk"], True, dh ** -0.5, 2.0 ** -8)
+    check([got], val, tol)
+    check([want], val, tol)
