@@ -38,6 +38,30 @@ template <typename T> __device__ __forceinline__ void row8(const T* x, int c, in
   for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < C ? to_f(x[8 * (int64_t)c + e]) : fill;
 }
 
+// the same 8 elements as they are stored, to be kept in registers between sweeps
+template <typename T> struct TopRaw8;
+template <> struct TopRaw8<bf16> {
+  bf16x8 t;
+  __device__ __forceinline__ void get(float v[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  }
+  __device__ __forceinline__ void set(int i, bf16 x) { t[i] = x; }
+};
+template <> struct TopRaw8<float> {
+  f32x4 t[2];
+  __device__ __forceinline__ void get(float v[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = t[i >> 2][i & 3];
+  }
+  __device__ __forceinline__ void set(int i, float x) { t[i >> 2][i & 3] = x; }
+};
+template <typename T> __device__ __forceinline__ void raw8(const T* x, int c, int C, float fill, TopRaw8<T>& o) {
+  if (8 * c + 8 <= C) { __builtin_memcpy(&o, x + 8 * (int64_t)c, sizeof(o)); return; }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o.set(e, 8 * c + e < C ? x[8 * (int64_t)c + e] : from_f<T>(fill));
+}
+
 // ---------------------------------------------------------------------------------------------
 // the k largest logits of a row
 // ---------------------------------------------------------------------------------------------
@@ -84,29 +108,30 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
   const T* x = logits + r * ld;
   const int chunks = (C + 7) >> 3;
   // rows of up to NCH * 8 * TOP_NT elements stay in registers between the sweeps (NCH = 0: longer ones are read again)
-  float keep[NCH > 0 ? NCH : 1][8];
+  TopRaw8<T> keep[NCH > 0 ? NCH : 1];
   if constexpr (NCH > 0) {
 #pragma unroll
-    for (int n = 0; n < NCH; ++n) {
-      const int c = tid + n * TOP_NT;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) keep[n][e] = -INFINITY;
-      if (c < chunks) row8<T>(x, c, C, -INFINITY, keep[n]);
-    }
+    for (int n = 0; n < NCH; ++n)
+      if (tid + n * TOP_NT < chunks) raw8<T>(x, tid + n * TOP_NT, C, -INFINITY, keep[n]);
   }
-  auto sweep = [&](auto f) {
+  auto again = [&](auto f) __attribute__((always_inline)) {
+    for (int c = tid; c < chunks; c += TOP_NT) {
+      float v[8];
+      row8<T>(x, c, C, -INFINITY, v);
+      f(v, 8 * c);
+    }
+  };
+  auto sweep = [&](auto f) __attribute__((always_inline)) {
     if constexpr (NCH > 0) {
 #pragma unroll
-      for (int n = 0; n < NCH; ++n) {
-        const int c = tid + n * TOP_NT;
-        if (c < chunks) f(keep[n], 8 * c);
-      }
+      for (int n = 0; n < NCH; ++n)
+        if (tid + n * TOP_NT < chunks) {
+          float v[8];
+          keep[n].get(v);
+          f(v, 8 * (tid + n * TOP_NT));
+        }
     } else {
-      for (int c = tid; c < chunks; c += TOP_NT) {
-        float v[8];
-        row8<T>(x, c, C, -INFINITY, v);
-        f(v, 8 * c);
-      }
+      again(f);
     }
   };
   float mx = -INFINITY;
@@ -158,7 +183,7 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
   if (n > TOP_CAP) {                                         // (block-uniform)
     auto reach = [&](uint32_t lo) {                          // elements with a key >= lo
       int m = 0;
-      sweep([&](const float (&v)[8], int i0) {
+      again([&](const float (&v)[8], int i0) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) m += (order_key(v[e]) >= lo && i0 + e < C) ? 1 : 0;
       });
@@ -174,7 +199,7 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
     while (lo < hi) {
       const int mid = lo + (hi - lo) / 2;
       int m = 0;
-      sweep([&](const float (&v)[8], int i0) {
+      again([&](const float (&v)[8], int i0) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) m += (order_key(v[e]) == v0 && i0 + e < mid && i0 + e < C) ? 1 : 0;
       });
@@ -183,7 +208,7 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
     __syncthreads();
     if (tid == 0) count = 0;
     __syncthreads();
-    sweep([&](const float (&v)[8], int i0) {
+    again([&](const float (&v)[8], int i0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t key = order_key(v[e]);

@@ -26,9 +26,9 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, co
     float v[8];
     load8<T>(xr + c * 8, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { const float t = v[e] - mean; q += t * t; }
+    for (int e = 0; e < 8; ++e) { const float t = v[e] - mean; q += mul_rn(t, t); }
   }
-  for (int i = (nchunk << 3) + lane; i < d; i += 64) { const float t = to_f(xr[i]) - mean; q += t * t; }
+  for (int i = (nchunk << 3) + lane; i < d; i += 64) { const float t = to_f(xr[i]) - mean; q += mul_rn(t, t); }
   const float rstd = rsqrtf(wave_sum(q) / (float)d + eps);
   T* yr = y + (size_t)row * d;
   for (int c = lane; c < nchunk; c += 64) {
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void ln_fwd_reg_kernel(const T* __restrict__ x
     for (int k = 0; k < DCH; ++k)
       if (lane + 64 * k < nchunk) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { const float t = v[k][e] - mean; q += t * t; }
+        for (int e = 0; e < 8; ++e) { const float t = v[k][e] - mean; q += mul_rn(t, t); }
       }
     const float rstd = rsqrtf(wave_sum(q) / (float)d + eps);
     T* yr = y + (size_t)row * d;
@@ -204,8 +204,8 @@ __global__ __launch_bounds__(256) void ln_fwd_pair768_kernel(const T* __restrict
     const float mean0 = wave_sum(s0) / (float)D, mean1 = wave_sum(s1) / (float)D;
 #pragma unroll
     for (int j = 0; j < 3; ++j) xc[j].opaque();
-    // (t * t rounded, then added: the one-row kernels' loops compile to a multiply and an add, and the outputs are to be theirs
-    // bit for bit - with two interleaved chains the compiler otherwise contracts SOME of these into fmas)
+    // (t * t rounded, then added, as in the one-row kernels: the outputs are to be theirs bit for bit, and left to itself the
+    // compiler contracts some of these into fmas)
     float q0 = 0.f, q1 = 0.f;
     {
       float v[8];

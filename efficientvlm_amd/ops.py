@@ -1496,33 +1496,45 @@ def cross_attention(q, kv, H, dh, scale, mask=None, gate=None, want_probs=True, 
 # ---------------------------------------------------------------------------------------------------
 def _on_device_of(t):
     """launches go to the device the tensors live on, whatever the current one is"""
-    return torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _raw_stream(t):
+    """the current stream of the tensor's device, as the C entries take it"""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _same_device(first, *others):
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
 
 
 def _heads3(x):
     """x [tokens, heads, dh] as the packed kernels read it: heads in whole 16-byte pieces, 16-byte aligned (slices of a packed
-    projection are; anything else is copied).  Returns (tensor, token stride, head stride)."""
-    unit = 16 // x.element_size()
-    st = [0 if n <= 1 else s for n, s in zip(x.shape[:2], x.stride()[:2])]
-    if (x.stride(2) != 1 and x.shape[2] > 1) or any(s % unit for s in st) or x.data_ptr() % 16:
+    projection are; anything else is copied).  Returns (tensor, address, token stride, head stride)."""
+    mask = 7 if x.dtype == torch.bfloat16 else 3
+    for _ in range(2):
+        n, h, _d = x.shape
+        st, sh, sd = x.stride()
+        st, sh, p = st if n > 1 else 0, sh if h > 1 else 0, x.data_ptr()
+        if sd == 1 and not ((st | sh) & mask or p & 15):
+            break
         x = x.clone(memory_format=torch.contiguous_format)
-        st = [0 if n <= 1 else s for n, s in zip(x.shape[:2], x.stride()[:2])]
-    return x, st[0], st[1]
+    return x, p, st, sh
 
 
 def _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal):
     """(args, tensors the pointers in them belong to) of one packed-attention launch"""
-    (q, qt, qh), (k, kt, kh), (v, vt, vh) = _heads3(q), _heads3(k), _heads3(v)
-    a = L.PackedAttnArgs(dtype=L.dt(q), Tq=q.shape[0], Tk=k.shape[0], S=cu_q.numel() - 1, H=q.shape[1], Hkv=k.shape[1],
-                         dh=q.shape[2], causal=int(bool(causal)), scale=scale, Q=L.ptr(q), K=L.ptr(k), V=L.ptr(v),
-                         q_tok=qt, q_head=qh, k_tok=kt, k_head=kh, v_tok=vt, v_head=vh,
-                         cu_q=L.ptr(cu_q), cu_k=L.ptr(cu_k), k_lens=L.ptr(k_lens))
+    (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = _heads3(q), _heads3(k), _heads3(v)
+    Tq, H, dh = q.shape
+    a = L.PackedAttnArgs(L.BF16 if q.dtype == torch.bfloat16 else L.F32, Tq, k.shape[0], cu_q.shape[0] - 1, H, k.shape[1], dh,
+                         causal, scale, qp, kp, vp, qt, qh, kt, kh, vt, vh, cu_q.data_ptr(), cu_k.data_ptr(),
+                         None if k_lens is None else k_lens.data_ptr())
     return a, (q, k, v)
 
 
@@ -1530,16 +1542,24 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, k_lens, scale, causal):
         need = any(ctx.needs_input_grad[:3])
+        lib = _lib()
         with _on_device_of(q):
             a, keep = _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal)
             Tq, H, dh = q.shape
-            O = torch.empty((Tq, H, dh), dtype=q.dtype, device=q.device)
-            lse = torch.empty((H, Tq), dtype=torch.float32, device=q.device) if need else None
-            lo = torch.empty_like(O) if need and q.dtype == torch.bfloat16 else None     # (what rounding took from O)
-            splits = _lib().evlm_packed_attention_splits(C.byref(a))
-            ws = torch.empty(splits * H * Tq * (dh + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-            a.O, a.O_lo, a.lse, a.workspace = L.ptr(O), L.ptr(lo), L.ptr(lse), L.ptr(ws)
-            L.check(_lib().evlm_packed_attention_fwd(C.byref(a), L.stream()), "packed_attention_fwd")
+            O = q.new_empty((Tq, H, dh))
+            lo = lse = ws = None
+            a.O = O.data_ptr()
+            if need:
+                lse = q.new_empty((H, Tq), dtype=torch.float32)
+                a.lse = lse.data_ptr()
+                if q.dtype == torch.bfloat16:                   # (what rounding takes from O)
+                    lo = torch.empty_like(O)
+                    a.O_lo = lo.data_ptr()
+            splits = lib.evlm_packed_attention_splits(C.byref(a))
+            if splits > 1:
+                ws = q.new_empty(splits * H * Tq * (dh + 2), dtype=torch.float32)
+                a.workspace = ws.data_ptr()
+            L.check(lib.evlm_packed_attention_fwd(C.byref(a), _raw_stream(q)), "packed_attention_fwd")
         if need:
             ctx.save_for_backward(*keep, cu_q, cu_k, k_lens, O, lo, lse)
             ctx.meta = (scale, causal)
@@ -1552,18 +1572,18 @@ class _PackedAttention(torch.autograd.Function):
         scale, causal = ctx.meta
         with _on_device_of(q):
             a, keep = _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal)
-            dO, ot, oh = _heads3(dO)
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            dO, a.dO, a.do_tok, a.do_head = _heads3(dO)
+            dq = q.new_empty(q.shape)
             # (the kernels write every key of every sequence and the rows outside all of them; unfilled room is left alone)
-            alloc = torch.empty if k_lens is None else torch.zeros
-            dk, dv = alloc(k.shape, dtype=k.dtype, device=k.device), alloc(v.shape, dtype=v.dtype, device=v.device)
+            dk, dv = (k.new_empty(k.shape), v.new_empty(k.shape)) if k_lens is None else (k.new_zeros(k.shape), v.new_zeros(k.shape))
             delta = torch.empty_like(lse)
-            a.O, a.O_lo, a.lse, a.delta, a.dO, a.do_tok, a.do_head = L.ptr(O), L.ptr(lo), L.ptr(lse), L.ptr(delta), L.ptr(dO), ot, oh
-            for name, t in (("dq", dq), ("dk", dk), ("dv", dv)):
-                setattr(a, "dQ" if name == "dq" else ("dK" if name == "dk" else "dV"), L.ptr(t))
-                setattr(a, name + "_tok", t.stride(0))
-                setattr(a, name + "_head", t.stride(1))
-            L.check(_lib().evlm_packed_attention_bwd(C.byref(a), L.stream()), "packed_attention_bwd")
+            a.O, a.lse, a.delta, a.dQ, a.dK, a.dV = O.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+            if lo is not None:
+                a.O_lo = lo.data_ptr()
+            _, H, dh = q.shape
+            a.dq_tok, a.dk_tok, a.dv_tok = H * dh, k.shape[1] * dh, k.shape[1] * dh
+            a.dq_head = a.dk_head = a.dv_head = dh
+            L.check(_lib().evlm_packed_attention_bwd(C.byref(a), _raw_stream(q)), "packed_attention_bwd")
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -1583,35 +1603,34 @@ def packed_attention(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=T
 
     The padded kinds are self_attention / cross_attention (with the probability map as an output); the decoder masks of
     eff_bert.py:975-996 are the causal form here."""
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise RuntimeError(f"packed_attention: {n} must be [tokens, heads, head dim], got {tuple(t.shape)}")
-        if t.dtype != q.dtype:
-            raise TypeError("packed_attention: q, k and v must have one dtype")
+    qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or len(vs) != 3:
+        raise RuntimeError(f"packed_attention: q, k and v must be [tokens, heads, head dim], got {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    if k.dtype != dt or v.dtype != dt:
+        raise TypeError("packed_attention: q, k and v must have one dtype")
     L.dt(q)
-    H, dh = q.shape[1], q.shape[2]
-    if k.shape != v.shape or k.shape[2] != dh:
-        raise RuntimeError(f"packed_attention: k {tuple(k.shape)} and v {tuple(v.shape)} must agree, with q's head dim {dh}")
-    Hkv = k.shape[1]
+    Tq, H, dh = qs
+    Tk, Hkv, _ = ks
+    if ks != vs or ks[2] != dh:
+        raise RuntimeError(f"packed_attention: k {tuple(ks)} and v {tuple(vs)} must agree, with q's head dim {dh}")
     if H == 0 or Hkv == 0 or H % Hkv:
         raise RuntimeError(f"packed_attention: {H} query heads are no multiple of {Hkv} key heads")
     if dh == 0 or dh > 128 or dh % 8:
         raise RuntimeError(f"packed_attention: head dim {dh} is not a multiple of 8 up to 128")
-    if max(q.shape[0], k.shape[0]) > 1 << 30:
+    if max(Tq, Tk) > 1 << 30:
         raise RuntimeError("packed_attention: more than 2^30 tokens")
     scale = dh ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise RuntimeError(f"packed_attention: the scale must be positive and finite, got {scale}")
     if cu_k is None:
         cu_k = cu_q
-        if k.shape[0] != q.shape[0]:
+        if Tk != Tq:
             raise RuntimeError("packed_attention: without cu_k there must be as many keys as queries")
-    for n, t in (("cu_q", cu_q), ("cu_k", cu_k), ("k_lens", k_lens)):
-        if t is None:
-            continue
+    for t in (cu_q, cu_k) if k_lens is None else (cu_q, cu_k, k_lens):
         if t.dtype != torch.int32 or t.dim() != 1:
-            raise TypeError(f"packed_attention: {n} must be a 1-d int32 tensor")
-    if cu_q.numel() < 1 or cu_k.numel() != cu_q.numel() or (k_lens is not None and k_lens.numel() != cu_q.numel() - 1):
+            raise TypeError("packed_attention: cu_q, cu_k and k_lens must be 1-d int32 tensors")
+    S = cu_q.shape[0] - 1
+    if S < 0 or cu_k.shape[0] != S + 1 or (k_lens is not None and k_lens.shape[0] != S):
         raise RuntimeError("packed_attention: cu_q and cu_k need S + 1 entries, k_lens S")
     _same_device(q, k, v, cu_q, cu_k, k_lens)
     L.require_cuda(q)
@@ -2558,7 +2577,7 @@ def _top_rows(x, name):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise RuntimeError(f"{name}: logits must be [..., classes], got {tuple(x.shape)}")
     Cn = x.shape[-1]
-    x2 = x.reshape(-1, Cn)
+    x2 = x if x.dim() == 2 else x.reshape(-1, Cn)
     if (x2.stride(1) != 1 and Cn > 1) or (x2.shape[0] > 1 and x2.stride(0) < Cn):
         x2 = x2.contiguous()
     return x2, x2.shape[0], Cn, x2.stride(0) if x2.shape[0] > 1 else Cn
@@ -2586,8 +2605,8 @@ def top_logits(logits, k, temperature=1.0):
         lse = torch.empty(lead, dtype=torch.float32, device=x.device)
         if lse.numel():
             x2, R, Cn, ld = _top_rows(x, "top_logits")
-            L.check(_lib().evlm_top_logits(L.dt(x2), L.ptr(x2), R, Cn, ld, k, 1.0 / T, L.ptr(values), L.ptr(classes),
-                                           L.ptr(lse), L.stream()), "top_logits")
+            L.check(_lib().evlm_top_logits(L.dt(x2), x2.data_ptr(), R, Cn, ld, k, 1.0 / T, values.data_ptr(),
+                                           classes.data_ptr(), lse.data_ptr(), _raw_stream(x)), "top_logits")
     return values, classes, lse
 
 
@@ -2597,11 +2616,13 @@ class _KLTop(torch.autograd.Function):
         with _on_device_of(s):
             s2, R, Cn, ld = _top_rows(s, "soft_cross_entropy_top")
             k = values.shape[-1]
-            out = torch.empty((), dtype=torch.float32, device=s.device)
-            work = torch.empty(8 * R, dtype=torch.float32, device=s.device)      # 7 statistics of each row, then the rows' losses
-            rowloss = C.c_void_p(work.data_ptr() + 28 * R)
-            L.check(_lib().evlm_kl_top_fwd(L.dt(s2), L.ptr(s2), R, Cn, ld, L.ptr(values), L.ptr(classes), L.ptr(lse), k, inv_t,
-                                           1.0, L.ptr(weight), L.ptr(work), rowloss, L.ptr(out), L.stream()), "kl_top_fwd")
+            out = values.new_empty(())
+            work = values.new_empty(8 * R)                   # 7 statistics of each row, then the rows' losses
+            wp = work.data_ptr()
+            L.check(_lib().evlm_kl_top_fwd(L.dt(s2), s2.data_ptr(), R, Cn, ld, values.data_ptr(), classes.data_ptr(),
+                                           None if lse is None else lse.data_ptr(), k, inv_t, 1.0,
+                                           None if weight is None else weight.data_ptr(), wp, wp + 28 * R, out.data_ptr(),
+                                           _raw_stream(s)), "kl_top_fwd")
         ctx.save_for_backward(s2, values, classes, weight, work)
         ctx.meta = (R, Cn, ld, k, inv_t, lse is not None, s.shape)
         ctx.join = getattr(s, "_evlm_join", None)
@@ -2613,13 +2634,12 @@ class _KLTop(torch.autograd.Function):
         s2, values, classes, weight, work = ctx.saved_tensors
         R, Cn, ld, k, inv_t, rest, shape = ctx.meta
         with _on_device_of(s2):
-            gc = g.to(torch.float32).contiguous()
             ldd = _pad8(Cn)
             acc, join = _join_target(ctx, R, ldd, s2.dtype)
-            ds = acc if acc is not None else torch.empty((R, ldd), dtype=s2.dtype, device=s2.device)   # (padding: zeroed by the kernel)
-            L.check(_lib().evlm_kl_top_bwd(L.dt(s2), L.ptr(s2), R, Cn, ld, L.ptr(values), L.ptr(classes), int(rest), k, inv_t,
-                                           1.0, L.ptr(weight), L.ptr(work), L.ptr(gc), L.ptr(ds), ldd, int(acc is not None),
-                                           L.stream()), "kl_top_bwd")
+            ds = acc if acc is not None else s2.new_empty((R, ldd))                    # (padding columns: zeroed by the kernel)
+            L.check(_lib().evlm_kl_top_bwd(L.dt(s2), s2.data_ptr(), R, Cn, ld, values.data_ptr(), classes.data_ptr(), int(rest), k,
+                                           inv_t, 1.0, None if weight is None else weight.data_ptr(), work.data_ptr(),
+                                           g.data_ptr(), ds.data_ptr(), ldd, int(acc is not None), _raw_stream(s2)), "kl_top_bwd")
         if acc is not None:
             return None, None, None, None, None, None
         d = ds[:, :Cn] if ldd != Cn else ds
