@@ -37,7 +37,8 @@ struct PkArgs {
   int Tq, Tk, S, H, G, dh;          // G = heads per key head
   int gp, chunks, units;            // heads packed into a row block, chunks of a group, chunks * key heads
   int per, tiles;                   // tokens (keys) of a block, grid tiles
-  int splits, causal;
+  int splits, causal;               // splits: forward, parts of the keys; backward, parts of the rows of a key block
+  unsigned inv_gp;                  // 2^16 / gp rounded up: r / gp = r * inv_gp >> 16 for r < 256
   float scale, c;                   // c = scale * log2e
 };
 
@@ -55,38 +56,57 @@ __device__ __forceinline__ f32x16 mma(const f32x4& a, const f32x4& b, f32x16 c) 
   return c;
 }
 
+// LDS addresses as numbers: all pieces of a row, and all column blocks of 4 rows, lie at base ^ (constant)
+typedef __attribute__((address_space(3))) const char* lds_ptr;
+__device__ __forceinline__ uint32_t lds_of(const char* p) { return (uint32_t)(uintptr_t)(lds_ptr)p; }
+template <typename F> __device__ __forceinline__ F lds_read(uint32_t at) { return *(__attribute__((address_space(3))) const F*)(uintptr_t)at; }
+
 // Row-major LDS tile [rows][D], 16-byte pieces of a row permuted so that neither the row reads (16 rows, one piece each) nor
-// the column reads (4 rows, a pair of pieces each) meet in a bank: pairs move by the low row bits, the pieces of a pair by bit 3.
+// the column reads (4 consecutive rows, 4 consecutive pieces each) of a half-wave meet in one of the 16 piece-wide bank groups:
+// the two low row bits move groups of 4 pieces, the next two the pieces within a group (128-byte rows: two rows share the
+// bank groups, the lowest row bit selects the half).  SQ_LDS_BANK_CONFLICT: 0.
 template <typename T, int D> struct Tile {
   typedef typename Frag<T>::type frag;
   static constexpr int RB = D * (int)sizeof(T), NC = RB / 16, NS = RB / 32, EP = 16 / (int)sizeof(T);
   static __device__ __forceinline__ int at(int row, int c) {
-    const int x = NC == 8 ? ((((row >> 1) & 3) << 1) | ((row >> 3) & 1)) : (((row & 7) << 1) | ((row >> 3) & 1));
+    const int x = NC == 8 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
     return row * RB + (c ^ x) * 16;
   }
   // 32 rows as columns of a product: lane -> row lane & 31, pieces 2s + (lane >> 5); null row: zeros
   static __device__ __forceinline__ void load_cols(const T* row, int dh, int hh, frag (&f)[NS]) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
+      f[s] = frag{};
       const int e = (2 * s + hh) * EP;
-      frag z = {};
-      f[s] = (row && e < dh) ? *reinterpret_cast<const frag*>(row + e) : z;
+      if (row && e < dh) f[s] = *reinterpret_cast<const frag*>(row + e);
     }
   }
   static __device__ __forceinline__ f32x16 row_mm(const char* tile, int r0, const frag (&b)[NS], int lane) {
     f32x16 acc = {};
-    const int row = r0 + (lane & 31), hh = lane >> 5;
+    const uint32_t base = lds_of(tile) + at(r0 + (lane & 31), lane >> 5);
 #pragma unroll
-    for (int s = 0; s < NS; ++s) acc = mma(*reinterpret_cast<const frag*>(tile + at(row, 2 * s + hh)), b[s], acc);
+    for (int s = 0; s < NS; ++s) acc = mma(lds_read<frag>(base ^ (32 * s)), b[s], acc);
     return acc;
   }
-  static __device__ __forceinline__ void col_mm(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane);
+  // NB blocks of 32 rows against the same columns
+  template <int NB> static __device__ __forceinline__ void rows_mm(const char* tile, const frag (&b)[NS], f32x16 (&acc)[NB], int lane) {
+    const uint32_t base = lds_of(tile) + at(lane & 31, lane >> 5);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[n] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) acc[n] = mma(lds_read<frag>((base ^ (32 * s)) + 32 * n * RB), b[s], acc[n]);
+  }
 };
 
+// acc[d][c] += sum_r tile[r][d] p[r][c]
 // bf16: register i of C holds tile row 8 (i >> 2) + 4 (lane >> 5) + (i & 3); registers 8kk .. 8kk + 7 are the B operand of k-step
 // kk, and the A operand takes its 8 rows in that order: two transposing reads of 4 rows x 16 columns each
-template <int D> __device__ __forceinline__ void col_mm_bf16(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+template <int D> __device__ __forceinline__ void col_mm(const bf16*, const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+  typedef Tile<bf16, D> TL;
   const int hh = lane >> 5, w = lane & 15, sub = (lane >> 4) & 1;
+  const uint32_t base = lds_of(tile) + TL::at(r0 + 4 * hh + (w >> 2), sub * 2 + ((w & 3) >> 1)) + (w & 1) * 8;
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
     bf16x8 b;
@@ -94,20 +114,18 @@ template <int D> __device__ __forceinline__ void col_mm_bf16(const char* tile, i
     for (int j = 0; j < 8; ++j) b[j] = (bf16)p[8 * kk + j];
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
-      const int c = dt * 4 + sub * 2 + ((w & 3) >> 1);
       bf16x8 a;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = r0 + 16 * kk + 8 * half + 4 * hh + (w >> 2);
+      for (int half = 0; half < 2; ++half) {                 // rows r0 + 16 kk + 8 half + 4 (lane >> 5) .. + 3, columns 32 dt ..
         const bf16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-            (bf16x4 __attribute__((address_space(3)))*)(tile + Tile<bf16, D>::at(row, c) + (w & 1) * 8));
+            (bf16x4 __attribute__((address_space(3)))*)(uintptr_t)((base ^ (64 * dt + 32 * half)) + (16 * kk + 8 * half) * TL::RB));
         a[4 * half + 0] = t[0]; a[4 * half + 1] = t[1]; a[4 * half + 2] = t[2]; a[4 * half + 3] = t[3];
       }
-      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[dt], 0, 0, 0);
+      acc[dt] = mma(a, b, acc[dt]);
     }
   }
 }
-template <int D> __device__ __forceinline__ void col_mm_f32(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+template <int D> __device__ __forceinline__ void col_mm(const float*, const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
   const int hh = lane >> 5, w = lane & 31;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -119,10 +137,6 @@ template <int D> __device__ __forceinline__ void col_mm_f32(const char* tile, in
       acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[i], acc[dt], 0, 0, 0);
     }
   }
-}
-template <typename T, int D> __device__ __forceinline__ void Tile<T, D>::col_mm(const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
-  if constexpr (sizeof(T) == 2) col_mm_bf16<D>(tile, r0, p, acc, lane);
-  else col_mm_f32<D>(tile, r0, p, acc, lane);
 }
 // C register -> row of the 32-row block
 __device__ __forceinline__ int c_row(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
@@ -139,14 +153,49 @@ __device__ __forceinline__ Seq load_seq(const PkArgs& a, int s) {
   if (a.k_lens) q.klen = clampi(a.k_lens[s], 0, q.klen);
   return q;
 }
+__device__ __forceinline__ Seq uniform(const Seq& x) {       // what every lane holds alike, in scalar registers
+  return Seq{__builtin_amdgcn_readfirstlane(x.qs), __builtin_amdgcn_readfirstlane(x.qlen), __builtin_amdgcn_readfirstlane(x.ks),
+             __builtin_amdgcn_readfirstlane(x.klen)};
+}
 __device__ __forceinline__ int vis_of(const PkArgs& a, const Seq& q, int tok) {
   return a.causal ? clampi(q.klen - q.qlen + tok + 1, 0, q.klen) : q.klen;
 }
-// Block t of all sequences' blocks in order (KEYS: of their keys): the sequence it belongs to and its index there.  Every wave
-// counts 64 sequences at a time.  False: t lies behind the last block (t - total in `over`), the block has nothing to do but the rows
-// outside all sequences.
+// Block t of all sequences' blocks (KEYS: of their keys): the sequence it belongs to and its index there.  False: t lies behind the last
+// block (t - total in `over`), the block has nothing to do but the rows outside all sequences.  Every wave counts 64 sequences
+// at a time.  Up to 64 causal sequences are taken longest blocks first - the j-th block of queries, or the j-th block of keys from
+// the end, of every sequence that has one, j descending - so that the chip does not end on a few long blocks; of more
+// sequences, one after the other.
 template <bool KEYS> __device__ __forceinline__ bool find_tile(const PkArgs& a, int t, Seq& q, int& i, int& over, int& total) {
   const int lane = threadIdx.x & 63;
+  if (a.causal && a.S <= 64) {
+    int n = 0;
+    if (lane < a.S) {
+      const Seq x = load_seq(a, lane);
+      n = ((KEYS ? x.klen : x.qlen) + a.per - 1) / a.per;
+    }
+    auto from = [&](int j) {                                 // blocks of a level >= j
+      int64_t f = max(0, n - j);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) f += __shfl_xor(f, o, 64);
+      return f;
+    };
+    int lo = 0, hi = n;                                      // level: the largest j with from(j) > t
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) hi = max(hi, __shfl_xor(hi, o, 64));
+    const int64_t all = from(0);
+    if (t >= all) { over = (int)(t - all); total = (int)all; return false; }
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (from(mid) > t) lo = mid; else hi = mid;
+    }
+    int64_t rank = t - from(lo + 1);
+    unsigned long long has = __ballot(n > lo);
+    for (; rank > 0; --rank) has &= has - 1;
+    const int s = __builtin_ctzll(has);
+    q = uniform(load_seq(a, s));
+    i = __builtin_amdgcn_readfirstlane(KEYS ? __shfl(n, s, 64) - 1 - lo : lo);
+    return true;
+  }
   int64_t before = 0;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     int n = 0;
@@ -164,8 +213,8 @@ template <bool KEYS> __device__ __forceinline__ bool find_tile(const PkArgs& a, 
     if (hit) {
       const int l = __builtin_ctzll(hit);
       const int64_t first = before + __shfl(incl - n, l, 64);
-      q = load_seq(a, s0 + l);
-      i = (int)(t - first);
+      q = uniform(load_seq(a, s0 + l));
+      i = __builtin_amdgcn_readfirstlane((int)(t - first));
       return true;
     }
     before += __shfl(incl, 63, 64);
@@ -188,24 +237,48 @@ template <typename T, int D, int ROWS, int NT> struct Stage {
   static constexpr int N = ROWS * TL::NC / NT;
   static_assert(ROWS * TL::NC % NT == 0, "whole pieces per thread");
   typename TL::frag v[N];
-  // rows first .. first + ROWS - 1 of `base` (row stride `stride` elements); rows >= n repeat row n - 1 (their scores are masked)
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int first, int n, int dh, int tid) {
+  // (no branch around a load: pieces behind the head dim read the row's first piece and are zeroed in registers)
+  __device__ __forceinline__ void pad(int dh, int tid) {
+    if (dh == D) return;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int id = tid + k * NT, row = min(first + id / TL::NC, n - 1), e = (id % TL::NC) * TL::EP;
-      typename TL::frag z = {};
-      v[k] = e < dh ? *reinterpret_cast<const typename TL::frag*>(base + row * stride + e) : z;
+    for (int k = 0; k < N; ++k)
+      if (((tid + k * NT) % TL::NC) * TL::EP >= dh) v[k] = typename TL::frag{};
+  }
+  // rows first .. first + ROWS - 1 of `base` (row stride `stride` elements, everything the same in all lanes): a scalar address for
+  // each piece plus one 32-bit offset of the thread.  Rows >= n repeat row n - 1 (their scores are masked)
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int first, int n, int dh, int tid) {
+    constexpr int RP = NT / TL::NC;                          // rows of one piece of the block
+    const int r = tid / TL::NC, e0 = (tid % TL::NC) * TL::EP, e = e0 < dh ? e0 : 0;
+    if (first + ROWS <= n) {
+      const uint32_t off = (uint32_t)(r * (int)stride + e) * (uint32_t)sizeof(T);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        v[k] = *reinterpret_cast<const typename TL::frag*>((const char*)(base + (int64_t)(first + k * RP) * stride) + off);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        v[k] = *reinterpret_cast<const typename TL::frag*>(base + min(first + k * RP + r, n - 1) * stride + e);
     }
   }
-  // packed rows: row r = (token first + r / gp, head r % gp), zeros behind the last token and in unused rows
+  // packed rows: row r = (token first + r / gp, head r % gp); rows behind the last token repeat it, unused rows are those of the
+  // tokens that follow (the row's lse of +inf makes its probabilities zero).  Where gp divides the rows of a piece, every piece
+  // is a scalar address plus the thread's one offset
   __device__ __forceinline__ void load_rows(const T* base, int64_t tok_stride, int64_t head_stride, int first, int qlen, int gp,
-                                            int rows_used, int dh, int tid) {
+                                            unsigned inv_gp, int dh, int tid) {
+    constexpr int RP = NT / TL::NC;
+    const int r0 = tid / TL::NC, e0 = (tid % TL::NC) * TL::EP, e = e0 < dh ? e0 : 0;
+    if ((gp & (gp - 1)) == 0 && gp <= RP && first + (int)((ROWS - 1) * inv_gp >> 16) < qlen) {
+      const int rt = (int)(r0 * inv_gp >> 16), step = (int)(RP * inv_gp >> 16);
+      const uint32_t off = (uint32_t)(rt * (int)tok_stride + (r0 - rt * gp) * (int)head_stride + e) * (uint32_t)sizeof(T);
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int id = tid + k * NT, r = id / TL::NC, e = (id % TL::NC) * TL::EP, tok = first + r / gp, h = r % gp;
-      typename TL::frag z = {};
-      v[k] = (e < dh && r < rows_used && tok < qlen)
-                 ? *reinterpret_cast<const typename TL::frag*>(base + tok * tok_stride + h * head_stride + e) : z;
+      for (int k = 0; k < N; ++k)
+        v[k] = *reinterpret_cast<const typename TL::frag*>((const char*)(base + (int64_t)(first + k * step) * tok_stride) + off);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int r = r0 + k * RP, rt = (int)(r * inv_gp >> 16), tok = min(first + rt, qlen - 1);
+        v[k] = *reinterpret_cast<const typename TL::frag*>(base + tok * tok_stride + (r - rt * gp) * head_stride + e);
+      }
     }
   }
   __device__ __forceinline__ void store(char* tile, int tid) const {
@@ -227,8 +300,7 @@ __device__ __forceinline__ void attend(const char* Ks, const char* Vs, int kt0, 
                                        f32x16 (&o)[D / 32], int lane) {
   const int hh = lane >> 5;
   f32x16 s[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) s[b] = Tile<T, D>::row_mm(Ks, 32 * b, qf, lane);
+  Tile<T, D>::template rows_mm<NB>(Ks, qf, s, lane);
   if (mask) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -259,7 +331,7 @@ __device__ __forceinline__ void attend(const char* Ks, const char* Vs, int kt0, 
       s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -mc));
       l += s[b][i];
     }
-    Tile<T, D>::col_mm(Vs, 32 * b, s[b], o, lane);
+    col_mm<D>((const T*)nullptr, Vs, 32 * b, s[b], o, lane);
   }
 }
 
@@ -311,9 +383,9 @@ template <typename T> __device__ __forceinline__ void fwd_outside(const PkArgs& 
 template <typename T, int D, int NW, int BN>
 __global__ __launch_bounds__(64 * NW, 2) void pk_fwd_rows_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
-  __shared__ __attribute__((aligned(16))) char sm[2 * BN * TL::RB];
+  __shared__ __attribute__((aligned(512))) char sm[2 * BN * TL::RB];
   char *Ks = sm, *Vs = sm + BN * TL::RB;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
   Seq q; int ti, over, total;
   if (!find_tile<false>(a, blockIdx.x / a.units, q, ti, over, total)) { fwd_outside<T>(a, h0, over, total); return; }
@@ -322,8 +394,9 @@ __global__ __launch_bounds__(64 * NW, 2) void pk_fwd_rows_kernel(PkArgs a) {
   const int vis = valid ? vis_of(a, q, tok) : 0;
   const int last = min(tok0 + a.per, q.qlen) - 1;
   const int nk = vis_of(a, q, last);                                                    // keys any row of the block sees
-  const int w_min = vis_of(a, q, min(tok0 + wave * 32 / a.gp, last)), w_max = vis_of(a, q, min(tok0 + (wave * 32 + 31) / a.gp, last));
-  const bool w_any = tok0 + wave * 32 / a.gp <= last;
+  const int w_lo = tok0 + (int)(wave * 32 * a.inv_gp >> 16), w_hi = tok0 + (int)((wave * 32 + 31) * a.inv_gp >> 16);      // the wave's tokens
+  const int w_min = vis_of(a, q, min(w_lo, last)), w_max = vis_of(a, q, min(w_hi, last));
+  const bool w_any = w_lo <= last;
   typename TL::frag qf[TL::NS];
   TL::load_cols(valid ? (const T*)a.Q + (q.qs + tok) * a.q_tok + h * a.q_head : nullptr, a.dh, hh, qf);
   const T* Kb = (const T*)a.K + q.ks * a.k_tok + kh * a.k_head;
@@ -334,6 +407,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pk_fwd_rows_kernel(PkArgs a) {
   if (nk > 0) { ks.load(Kb, a.k_tok, 0, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, 0, q.klen, a.dh, tid); }
   for (int kt = 0; kt < nk; kt += BN) {
     __syncthreads();
+    ks.pad(a.dh, tid); vs.pad(a.dh, tid);
     ks.store(Ks, tid); vs.store(Vs, tid);
     __syncthreads();
     if (kt + BN < nk) { ks.load(Kb, a.k_tok, kt + BN, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, kt + BN, q.klen, a.dh, tid); }
@@ -361,9 +435,9 @@ template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
   constexpr int WB = 2 * 32 * TL::RB > 32 * D * 4 ? 2 * 32 * TL::RB : 32 * D * 4;       // one wave's tiles, later its context
-  __shared__ __attribute__((aligned(16))) char sm[NW * WB];
+  __shared__ __attribute__((aligned(512))) char sm[NW * WB];
   __shared__ float sml[NW][2][32];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
   const int rest = blockIdx.x / a.units, split = rest % a.splits;
   Seq q; int ti, over, total;
@@ -391,6 +465,7 @@ __global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
   if (kb < b1) { ks.load(Kb, a.k_tok, kb * 32, q.klen, a.dh, lane); vs.load(Vb, a.v_tok, kb * 32, q.klen, a.dh, lane); }
   for (; kb < b1; kb += NW) {
     wave_lds_fence();
+    ks.pad(a.dh, lane); vs.pad(a.dh, lane);
     ks.store(Ks, lane); vs.store(Vs, lane);
     wave_lds_fence();
     if (kb + NW < b1) {
@@ -504,9 +579,9 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
 template <typename T, int D, int NW, int BN>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
-  __shared__ __attribute__((aligned(16))) char sm[2 * BN * TL::RB];
+  __shared__ __attribute__((aligned(512))) char sm[2 * BN * TL::RB];
   char *Ks = sm, *Vs = sm + BN * TL::RB;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
   Seq q; int ti, over, total;
   if (!find_tile<false>(a, blockIdx.x / a.units, q, ti, over, total)) {
@@ -520,8 +595,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
   const int vis = valid ? vis_of(a, q, tok) : 0;
   const int last = min(tok0 + a.per, q.qlen) - 1;
   const int nk = vis_of(a, q, last);
-  const int w_min = vis_of(a, q, min(tok0 + wave * 32 / a.gp, last)), w_max = vis_of(a, q, min(tok0 + (wave * 32 + 31) / a.gp, last));
-  const bool w_any = tok0 + wave * 32 / a.gp <= last;
+  const int w_lo = tok0 + (int)(wave * 32 * a.inv_gp >> 16), w_hi = tok0 + (int)((wave * 32 + 31) * a.inv_gp >> 16);      // the wave's tokens
+  const int w_min = vis_of(a, q, min(w_lo, last)), w_max = vis_of(a, q, min(w_hi, last));
+  const bool w_any = w_lo <= last;
   const int64_t t = q.qs + tok;
   typename TL::frag qf[TL::NS], df[TL::NS];
   TL::load_cols(valid ? (const T*)a.Q + t * a.q_tok + h * a.q_head : nullptr, a.dh, hh, qf);
@@ -552,6 +628,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
   if (nk > 0) { ks.load(Kb, a.k_tok, 0, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, 0, q.klen, a.dh, tid); }
   for (int kt = 0; kt < nk; kt += BN) {
     __syncthreads();
+    ks.pad(a.dh, tid); vs.pad(a.dh, tid);
     ks.store(Ks, tid); vs.store(Vs, tid);
     __syncthreads();
     if (kt + BN < nk) { ks.load(Kb, a.k_tok, kt + BN, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, kt + BN, q.klen, a.dh, tid); }
@@ -561,14 +638,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
       for (int b = 0; b < BN / 32; ++b) {
         f32x16 s = TL::row_mm(Ks, 32 * b, qf, lane);
         const f32x16 dp = TL::row_mm(Vs, 32 * b, df, lane);
+        if (mask) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse));
-          if (mask) p = kt + 32 * b + c_row(i, hh) < vis ? p : 0.f;
-          s[i] = p * (dp[i] - delta);
-          if (mask) s[i] = kt + 32 * b + c_row(i, hh) < vis ? s[i] : 0.f;
+          for (int i = 0; i < 16; ++i) s[i] = kt + 32 * b + c_row(i, hh) < vis ? s[i] : -INFINITY;
         }
-        TL::col_mm(Ks, 32 * b, s, acc, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * (dp[i] - delta);
+        col_mm<D>((const T*)nullptr, Ks, 32 * b, s, acc, lane);
       }
     }
   }
@@ -576,94 +652,174 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward, dK / dV: NW * 32 keys of one (sequence, key head); the rows of every head of the group stream through LDS
+// backward, dK / dV.  A wave holds 32 keys as columns; the NW waves are NW / RG groups of keys x RG groups of rows, whose sums are
+// joined at the end.  The rows of every head of the group stream through LDS, RG * RB * 32 at a time: a wave takes RB blocks of 32
+// between two barriers, so that the products of one and the exponentials of the other can overlap.  `splits` blocks share the
+// rows of a key block and leave f32 parts (joined by pk_bwd_join_kernel) where there are few key blocks.
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int NW, int BR>
-__global__ __launch_bounds__(64 * NW, 1) void pk_bwd_dkv_kernel(PkArgs a) {
+template <typename T, int D, int NW, int RG, int RB>
+__global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 ? 2 : 1) void pk_bwd_dkv_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
-  __shared__ __attribute__((aligned(16))) char sm[2 * BR * TL::RB];
+  constexpr int BR = 32 * RG * RB, KG = NW / RG, JOIN = KG * (RG - 1) * 32 * D * 4;
+  constexpr int SM = 2 * BR * TL::RB > JOIN ? 2 * BR * TL::RB : JOIN;
+  __shared__ __attribute__((aligned(512))) char sm[SM];
   __shared__ __attribute__((aligned(16))) float Ls[BR], Ds[BR];
   __shared__ __attribute__((aligned(16))) int Vis[BR];
   char *Qs = sm, *Os = sm + BR * TL::RB;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, kg = wave / RG, rg = wave % RG;
   const int nkh = a.H / a.G, kh = blockIdx.x % nkh;
+  const int rest = blockIdx.x / nkh, part = rest % a.splits;
   Seq q; int ti, over, total;
-  if (!find_tile<true>(a, blockIdx.x / nkh, q, ti, over, total)) {
-    outside_rows(a.cu_k, a.S, a.Tk, over, a.tiles - total, [&](int r) {
-      zero_row<T>((T*)a.dK + r * a.dk_tok + kh * a.dk_head, a.dh);
-      zero_row<T>((T*)a.dV + r * a.dv_tok + kh * a.dv_head, a.dh);
-    });
+  if (!find_tile<true>(a, rest / a.splits, q, ti, over, total)) {
+    if (a.splits == 1)
+      outside_rows(a.cu_k, a.S, a.Tk, over, a.tiles - total, [&](int r) {
+        zero_row<T>((T*)a.dK + r * a.dk_tok + kh * a.dk_head, a.dh);
+        zero_row<T>((T*)a.dV + r * a.dv_tok + kh * a.dv_head, a.dh);
+      });
     return;
   }
-  const int k0 = ti * a.per, key = k0 + wave * 32 + (lane & 31);
-  const bool valid = key < q.klen;
-  const bool w_any = k0 + wave * 32 < q.klen;
+  const int k0 = ti * a.per, w0 = k0 + kg * 32, key = w0 + (lane & 31);       // first key of the block, of the wave; the lane's
   typename TL::frag kf[TL::NS], vf[TL::NS];
-  TL::load_cols(valid ? (const T*)a.K + (q.ks + (int64_t)key) * a.k_tok + kh * a.k_head : nullptr, a.dh, hh, kf);
-  TL::load_cols(valid ? (const T*)a.V + (q.ks + (int64_t)key) * a.v_tok + kh * a.v_head : nullptr, a.dh, hh, vf);
+  TL::load_cols(key < q.klen ? (const T*)a.K + (q.ks + (int64_t)key) * a.k_tok + kh * a.k_head : nullptr, a.dh, hh, kf);
+  TL::load_cols(key < q.klen ? (const T*)a.V + (q.ks + (int64_t)key) * a.v_tok + kh * a.v_head : nullptr, a.dh, hh, vf);
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
-  const int btok = BR / a.gp, used = btok * a.gp;
-  // first query that sees key k0
+  const int btok = (int)(BR * a.inv_gp >> 16), used = btok * a.gp;
+  // row blocks: the tokens from the first that sees key k0, for one chunk of heads after the other
   const int first = a.causal ? max(0, k0 - (q.klen - q.qlen)) : 0;
+  const int per_chunk = first < q.qlen ? (q.qlen - first + btok - 1) / btok : 0;
+  const int64_t blocks = (int64_t)per_chunk * a.chunks;
+  const int b0 = (int)(blocks * part / a.splits), b1 = (int)(blocks * (part + 1) / a.splits);
+  int ch = per_chunk ? b0 / per_chunk : 0, tok0 = first + (b0 - ch * per_chunk) * btok;
   Stage<T, D, BR, 64 * NW> qs, os;
-  for (int ch = 0; ch < a.chunks; ++ch) {
-    const int h0 = kh * a.G + ch * a.gp;
-    const T* Qb = (const T*)a.Q + q.qs * a.q_tok + h0 * a.q_head;
-    const T* Ob = (const T*)a.dO + q.qs * a.do_tok + h0 * a.do_head;
-    float lv = INFINITY, dl = 0.f; int vi = 0;
-    auto load = [&](int tok0) {
-      qs.load_rows(Qb, a.q_tok, a.q_head, tok0, q.qlen, a.gp, used, a.dh, tid);
-      os.load_rows(Ob, a.do_tok, a.do_head, tok0, q.qlen, a.gp, used, a.dh, tid);
-      if (tid < BR) {
-        const int tok = tok0 + tid / a.gp;
-        const bool in = tid < used && tok < q.qlen;
-        const int64_t at = (int64_t)(h0 + tid % a.gp) * a.Tq + q.qs + tok;
-        lv = in ? a.lse[at] : INFINITY;
-        dl = in ? a.delta[at] : 0.f;
-        vi = in ? vis_of(a, q, tok) : 0;
-      }
-    };
-    if (first < q.qlen) load(first);
-    for (int tok0 = first; tok0 < q.qlen; tok0 += btok) {
-      __syncthreads();
-      qs.store(Qs, tid); os.store(Os, tid);
-      if (tid < BR) { Ls[tid] = lv; Ds[tid] = dl; Vis[tid] = vi; }
-      __syncthreads();
-      if (tok0 + btok < q.qlen) load(tok0 + btok);
-      // rows see every key of the wave's block unless the block crosses the diagonal or the end
-      const bool mask = (a.causal && vis_of(a, q, tok0) < k0 + wave * 32 + 32) || k0 + wave * 32 + 32 > q.klen;
-      const bool seen = w_any && vis_of(a, q, min(tok0 + btok, q.qlen) - 1) > k0 + wave * 32;
-      if (seen) {
+  float lv = INFINITY, dl = 0.f;
+  int vi = 0;
+  auto load = [&](int c, int t0) {
+    const int h0 = kh * a.G + c * a.gp;
+    qs.load_rows((const T*)a.Q + q.qs * a.q_tok + h0 * a.q_head, a.q_tok, a.q_head, t0, q.qlen, a.gp, a.inv_gp, a.dh, tid);
+    os.load_rows((const T*)a.dO + q.qs * a.do_tok + h0 * a.do_head, a.do_tok, a.do_head, t0, q.qlen, a.gp, a.inv_gp, a.dh, tid);
+    if (tid < BR) {
+      const int rt = (int)(tid * a.inv_gp >> 16), tok = t0 + rt;
+      const bool in = tid < used && tok < q.qlen;
+      const int64_t at = (int64_t)(h0 + tid - rt * a.gp) * a.Tq + q.qs + tok;
+      lv = in ? a.lse[at] : INFINITY;
+      dl = in ? a.delta[at] : 0.f;
+      vi = in ? vis_of(a, q, tok) : 0;
+    }
+  };
+  if (b0 < b1) load(ch, tok0);
+  for (int b = b0; b < b1; ++b) {
+    __syncthreads();
+    qs.pad(a.dh, tid); os.pad(a.dh, tid);
+    qs.store(Qs, tid); os.store(Os, tid);
+    if (tid < BR) { Ls[tid] = lv; Ds[tid] = dl; Vis[tid] = vi; }
+    __syncthreads();
+    const int now = tok0;
+    tok0 += btok;
+    if (tok0 >= q.qlen) { tok0 = first; ++ch; }
+    if (b + 1 < b1) load(ch, tok0);
+    // this wave's rows: tokens t_lo .. t_hi of the block.  Nothing to do if the last of them sees none of the wave's keys; masked
+    // if the first does not see all of them (columns behind the last key are not stored)
+    const int r_lo = 32 * RB * rg;
+    const int t_lo = now + (int)(r_lo * a.inv_gp >> 16), t_hi = min(now + (int)((r_lo + 32 * RB - 1) * a.inv_gp >> 16), q.qlen - 1);
+    if (t_lo >= q.qlen || vis_of(a, q, t_hi) <= w0) continue;
+    const bool mask = a.causal && vis_of(a, q, t_lo) < w0 + 32;
+    f32x16 p[RB], ds[RB];
 #pragma unroll
-        for (int b = 0; b < BR / 32; ++b) {
-          f32x16 p = TL::row_mm(Qs, 32 * b, kf, lane);
-          f32x16 ds = TL::row_mm(Os, 32 * b, vf, lane);
+    for (int n = 0; n < RB; ++n) {
+      p[n] = TL::row_mm(Qs, r_lo + 32 * n, kf, lane);
+      ds[n] = TL::row_mm(Os, r_lo + 32 * n, vf, lane);
+    }
+    if (mask) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r0 = 32 * b + 8 * j + 4 * hh;
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(Ls + r0), d4 = *reinterpret_cast<const f32x4*>(Ds + r0);
+      for (int n = 0; n < RB; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int i = 4 * j + e;
-              float x = __builtin_amdgcn_exp2f(fmaf(p[i], a.c, -l4[e]));
-              float y = x * (ds[i] - d4[e]);
-              if (mask) {
-                const bool in = valid && key < Vis[r0 + e];
-                x = in ? x : 0.f; y = in ? y : 0.f;
-              }
-              p[i] = x; ds[i] = y;
-            }
-          }
-          TL::col_mm(Os, 32 * b, p, dv, lane);
-          TL::col_mm(Qs, 32 * b, ds, dk, lane);
+        for (int i = 0; i < 16; ++i) p[n][i] = key < Vis[r_lo + 32 * n + c_row(i, hh)] ? p[n][i] : -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < RB; ++n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r0 = r_lo + 32 * n + 8 * j + 4 * hh;
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(Ls + r0), d4 = *reinterpret_cast<const f32x4*>(Ds + r0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * j + e;
+          const float x = __builtin_amdgcn_exp2f(fmaf(p[n][i], a.c, -l4[e]));
+          ds[n][i] = x * (ds[n][i] - d4[e]);
+          p[n][i] = x;
         }
       }
+      col_mm<D>((const T*)nullptr, Os, r_lo + 32 * n, p[n], dv, lane);
+      col_mm<D>((const T*)nullptr, Qs, r_lo + 32 * n, ds[n], dk, lane);
     }
   }
-  if (!valid) return;
+  if constexpr (RG > 1) {                                     // join the row groups, dK first, then dV
+    auto join = [&](f32x16 (&acc)[D / 32]) {
+      float* buf = (float*)sm + (size_t)kg * (RG - 1) * (D / 32) * 16 * 64;
+      __syncthreads();
+      if (rg > 0) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) buf[(((rg - 1) * (D / 32) + dt) * 16 + i) * 64 + lane] = acc[dt][i];
+      }
+      __syncthreads();
+      if (rg == 0) {
+#pragma unroll
+        for (int g = 0; g < RG - 1; ++g)
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] += buf[((g * (D / 32) + dt) * 16 + i) * 64 + lane];
+      }
+    };
+    join(dk);
+    join(dv);
+    if (rg > 0) return;
+  }
+  if (key >= q.klen) return;
   const int64_t kr = q.ks + (int64_t)key;
-  store_cols<T, D>((T*)a.dK + kr * a.dk_tok + kh * a.dk_head, a.dh, dk, a.scale, hh);
-  store_cols<T, D>((T*)a.dV + kr * a.dv_tok + kh * a.dv_head, a.dh, dv, 1.0f, hh);
+  if (a.splits > 1) {
+    float* o = a.part + ((((int64_t)part * 2) * a.Tk + kr) * nkh + kh) * a.dh;
+    store_cols<float, D>(o, a.dh, dk, a.scale, hh);
+    store_cols<float, D>(o + (int64_t)a.Tk * nkh * a.dh, a.dh, dv, 1.0f, hh);
+  } else {
+    store_cols<T, D>((T*)a.dK + kr * a.dk_tok + kh * a.dk_head, a.dh, dk, a.scale, hh);
+    store_cols<T, D>((T*)a.dV + kr * a.dv_tok + kh * a.dv_head, a.dh, dv, 1.0f, hh);
+  }
+}
+// sum of the parts, in order; one block of 256 threads per key (all heads, dK and dV).  Keys of no sequence: zeros
+template <typename T> __global__ __launch_bounds__(256) void pk_bwd_join_kernel(PkArgs a) {
+  const int64_t key = blockIdx.x;
+  const int nkh = a.H / a.G, row = nkh * a.dh;
+  // last sequence that starts at or before this key
+  int lo = 0, hi = a.S;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_k[mid] <= key) lo = mid + 1; else hi = mid;
+  }
+  const int s = lo - 1;
+  bool inside = false, room = false;
+  if (s >= 0) {
+    const Seq q = load_seq(a, s);
+    inside = key >= q.ks && key < (int64_t)q.ks + q.klen;
+    room = !inside && key < a.cu_k[s + 1];                    // (the unfilled part of a slot is left as it is)
+  }
+  if (room) return;
+  const int64_t plane = (int64_t)a.Tk * row;
+  for (int e = threadIdx.x * 4; e < 2 * row; e += 1024) {
+    const int which = e >= row, c = e - which * row, kh = c / a.dh, d = c - kh * a.dh;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (inside)
+      for (int p = 0; p < a.splits; ++p) {
+        float x[4];
+        Vec4<float>::load(a.part + (int64_t)(2 * p + which) * plane + key * row + c, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += x[j];
+      }
+    T* o = which ? (T*)a.dV + key * a.dv_tok + kh * a.dv_head : (T*)a.dK + key * a.dk_tok + kh * a.dk_head;
+    Vec4<T>::store(o + d, v);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -686,6 +842,18 @@ static int pk_splits(const evlm_packed_attn_args* x, int gp) {
   if (n > keys / 256) n = keys / 256;
   return n < 1 ? 1 : (n > 64 ? 64 : (int)n);
 }
+// dK / dV: row groups of a block of 4 waves; it covers 128 / groups keys
+static constexpr int pk_row_groups(int bytes, int D) { return bytes == 4 ? 1 : (D == 64 ? 4 : 2); }
+static bool pk_few_keys(const evlm_packed_attn_args* x) { return (int64_t)x->Tk <= (int64_t)48 * x->S; }
+// ... parts of the rows of a key block, where there are too few key blocks for the chip; each part still has some hundred rows
+static int pk_parts(const evlm_packed_attn_args* x) {
+  if (x->S == 0 || x->Tk == 0 || pk_few_keys(x)) return 1;
+  const int keys = 128 / pk_row_groups(x->dtype == EVLM_BF16 ? 2 : 4, x->dh <= 64 ? 64 : 128);
+  const int64_t blocks = ((int64_t)x->Tk / keys + x->S) * x->Hkv, rows = (int64_t)x->Tq * (x->H / x->Hkv) / x->S;
+  int64_t n = (256 + blocks - 1) / blocks;
+  if (n > rows / 512) n = rows / 512;
+  return n < 1 ? 1 : (n > 8 ? 8 : (int)n);
+}
 static int pk_check(const evlm_packed_attn_args* x, const char* name) {
   EVLM_REQUIRE(x->dtype == EVLM_F32 || x->dtype == EVLM_BF16, "%s: bad dtype %d", name, x->dtype);
   EVLM_REQUIRE(x->Tq >= 0 && x->Tk >= 0 && x->S >= 0 && x->H > 0 && x->Hkv > 0 && x->H % x->Hkv == 0, "%s: bad sizes", name);
@@ -696,6 +864,8 @@ static int pk_check(const evlm_packed_attn_args* x, const char* name) {
   const int64_t st[6] = {x->q_tok, x->q_head, x->k_tok, x->k_head, x->v_tok, x->v_head};
   const int unit = x->dtype == EVLM_BF16 ? 8 : 4;
   for (int i = 0; i < 6; ++i) EVLM_REQUIRE(st[i] >= 0 && st[i] % unit == 0, "%s: strides must be whole 16-byte pieces", name);
+  EVLM_REQUIRE(x->k_tok < (1 << 22) && x->v_tok < (1 << 22), "%s: token strides of K and V must stay below 2^22 elements", name);
+  EVLM_REQUIRE(x->q_tok < (1 << 22) && x->q_head < (1 << 22), "%s: strides of Q must stay below 2^22 elements", name);
   EVLM_REQUIRE((((uintptr_t)x->Q | (uintptr_t)x->K | (uintptr_t)x->V) & 15) == 0, "%s: tensors must be 16-byte aligned", name);
   return 0;
 }
@@ -706,19 +876,19 @@ static PkArgs pk_args(const evlm_packed_attn_args* x) {
   a.q_tok = x->q_tok; a.q_head = x->q_head; a.k_tok = x->k_tok; a.k_head = x->k_head; a.v_tok = x->v_tok; a.v_head = x->v_head;
   a.Tq = x->Tq; a.Tk = x->Tk; a.S = x->S; a.H = x->H; a.G = x->H / x->Hkv; a.dh = x->dh;
   a.gp = largest_divisor(a.G, 32);
+  a.inv_gp = (65536u + a.gp - 1) / a.gp;
   a.chunks = a.G / a.gp; a.units = a.chunks * x->Hkv;
   a.causal = x->causal != 0; a.scale = x->scale; a.c = x->scale * PK_LOG2E;
   a.splits = 1;
   return a;
 }
 // grid: `units` x (upper bound of the number of blocks + 1, so that there always is a surplus block for the rows outside)
-static int pk_grid(PkArgs& a, int rows, int64_t T, int per, int units, const char* name, unsigned* grid) {
+static int pk_grid(PkArgs& a, int64_t T, int per, int units, const char* name, unsigned* grid) {
   a.per = per;
   const int64_t tiles = T / per + a.S + 1, n = tiles * units * a.splits;
   if (n > 0x7fffffffll) return evlm_set_error("%s: too many blocks", name);
   a.tiles = (int)tiles;
   *grid = (unsigned)n;
-  (void)rows;
   return 0;
 }
 
@@ -727,11 +897,16 @@ extern "C" int evlm_packed_attention_splits(const evlm_packed_attn_args* x) {
   return pk_splits(x, largest_divisor(x->H / x->Hkv, 32));
 }
 
+extern "C" int evlm_packed_attention_bwd_parts(const evlm_packed_attn_args* x) {
+  if (!x || x->H <= 0 || x->Hkv <= 0 || x->H % x->Hkv) return 1;
+  return pk_parts(x);
+}
+
 template <typename T, int D> static int pk_fwd_launch(PkArgs& a, bool few, hipStream_t stream) {
   unsigned grid;
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   if (few) {
-    if (int rc = pk_grid(a, 32, a.Tq, 32 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
+    if (int rc = pk_grid(a, a.Tq, 32 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
     if (a.splits == 1 && a.S > 0 && a.Tk / a.S <= 64)
       hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 1>), dim3(grid), dim3(64), 0, stream, a);
     else
@@ -742,7 +917,7 @@ template <typename T, int D> static int pk_fwd_launch(PkArgs& a, bool few, hipSt
       hipLaunchKernelGGL((pk_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
     }
   } else {
-    if (int rc = pk_grid(a, 128, a.Tq, 128 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
+    if (int rc = pk_grid(a, a.Tq, 128 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
     hipLaunchKernelGGL((pk_fwd_rows_kernel<T, D, 4, BN>), dim3(grid), dim3(256), 0, stream, a);
   }
   EVLM_LAUNCH_CHECK("evlm_packed_attention_fwd");
@@ -769,28 +944,34 @@ extern "C" int evlm_packed_attention_fwd(const evlm_packed_attn_args* x, void* s
   return PK_DISPATCH(x, pk_fwd_launch)(a, few, (hipStream_t)stream_);
 }
 
-template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, hipStream_t stream) {
+template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, bool few_keys, int parts, hipStream_t stream) {
   unsigned grid;
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   const char* name = "evlm_packed_attention_bwd";
   const int nkh = a.H / a.G;
   if (a.Tq > 0) {
     if (few) {
-      if (int rc = pk_grid(a, 32, a.Tq, 32 / a.gp, a.units, name, &grid)) return rc;
+      if (int rc = pk_grid(a, a.Tq, 32 / a.gp, a.units, name, &grid)) return rc;
       hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 1, 32>), dim3(grid), dim3(64), 0, stream, a);
     } else {
-      if (int rc = pk_grid(a, 128, a.Tq, 128 / a.gp, a.units, name, &grid)) return rc;
+      if (int rc = pk_grid(a, a.Tq, 128 / a.gp, a.units, name, &grid)) return rc;
       hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 4, BN>), dim3(grid), dim3(256), 0, stream, a);
     }
     EVLM_LAUNCH_CHECK(name);
   }
   if (a.Tk > 0) {
-    if (a.S > 0 && a.Tk / a.S <= 48) {
-      if (int rc = pk_grid(a, 32, a.Tk, 32, nkh, name, &grid)) return rc;
-      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 1, 32>), dim3(grid), dim3(64), 0, stream, a);
+    a.splits = parts;
+    if (few_keys) {
+      if (int rc = pk_grid(a, a.Tk, 32, nkh, name, &grid)) return rc;
+      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 1, 1, 1>), dim3(grid), dim3(64), 0, stream, a);
     } else {
-      if (int rc = pk_grid(a, 128, a.Tk, 128, nkh, name, &grid)) return rc;
-      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 4, 32>), dim3(grid), dim3(256), 0, stream, a);
+      constexpr int RG = pk_row_groups((int)sizeof(T), D);
+      if (int rc = pk_grid(a, a.Tk, 128 / RG, nkh, name, &grid)) return rc;
+      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 4, RG, (sizeof(T) == 2 && D == 128 ? 2 : 1)>), dim3(grid), dim3(256), 0, stream, a);
+    }
+    if (a.splits > 1) {
+      EVLM_LAUNCH_CHECK(name);
+      hipLaunchKernelGGL((pk_bwd_join_kernel<T>), dim3((unsigned)a.Tk), dim3(256), 0, stream, a);
     }
     EVLM_LAUNCH_CHECK(name);
   }
@@ -808,10 +989,16 @@ extern "C" int evlm_packed_attention_bwd(const evlm_packed_attn_args* x, void* s
   const int unit = x->dtype == EVLM_BF16 ? 8 : 4;
   for (int i = 0; i < 8; ++i) EVLM_REQUIRE(st[i] >= 0 && st[i] % unit == 0, "%s: strides must be whole 16-byte pieces", name);
   EVLM_REQUIRE((((uintptr_t)x->dO | (uintptr_t)x->dQ | (uintptr_t)x->dK | (uintptr_t)x->dV) & 15) == 0, "%s: tensors must be 16-byte aligned", name);
+  EVLM_REQUIRE(x->do_tok < (1 << 22) && x->do_head < (1 << 22), "%s: strides of dO must stay below 2^22 elements", name);
   PkArgs a = pk_args(x);
   a.dO = x->dO; a.dQ = x->dQ; a.dK = x->dK; a.dV = x->dV; a.delta = x->delta;
   a.do_tok = x->do_tok; a.do_head = x->do_head; a.dq_tok = x->dq_tok; a.dq_head = x->dq_head;
   a.dk_tok = x->dk_tok; a.dk_head = x->dk_head; a.dv_tok = x->dv_tok; a.dv_head = x->dv_head;
   const bool few = x->S > 0 && pk_few_rows(x, a.gp);
-  return PK_DISPATCH(x, pk_bwd_launch)(a, few, (hipStream_t)stream_);
+  const int parts = pk_parts(x);
+  if (parts > 1) {
+    EVLM_REQUIRE(x->workspace, "%s: %d row parts need a workspace", name, parts);
+    a.part = (float*)x->workspace;
+  }
+  return PK_DISPATCH(x, pk_bwd_launch)(a, few, x->S > 0 && pk_few_keys(x), parts, (hipStream_t)stream_);
 }

@@ -1515,14 +1515,14 @@ def _same_device(first, *others):
 
 
 def _heads3(x):
-    """x [tokens, heads, dh] as the packed kernels read it: heads in whole 16-byte pieces, 16-byte aligned (slices of a packed
-    projection are; anything else is copied).  Returns (tensor, address, token stride, head stride)."""
+    """x [tokens, heads, dh] as the packed kernels read it: heads in whole 16-byte pieces, 16-byte aligned, strides below 2^22
+    elements (slices of a packed projection are; anything else is copied).  Returns (tensor, address, token stride, head stride)."""
     mask = 7 if x.dtype == torch.bfloat16 else 3
     for _ in range(2):
         n, h, _d = x.shape
         st, sh, sd = x.stride()
         st, sh, p = st if n > 1 else 0, sh if h > 1 else 0, x.data_ptr()
-        if sd == 1 and not ((st | sh) & mask or p & 15):
+        if sd == 1 and not ((st | sh) & mask or p & 15 or max(st, sh) >= 1 << 22):
             break
         x = x.clone(memory_format=torch.contiguous_format)
     return x, p, st, sh
@@ -1583,7 +1583,12 @@ class _PackedAttention(torch.autograd.Function):
             _, H, dh = q.shape
             a.dq_tok, a.dk_tok, a.dv_tok = H * dh, k.shape[1] * dh, k.shape[1] * dh
             a.dq_head = a.dk_head = a.dv_head = dh
-            L.check(_lib().evlm_packed_attention_bwd(C.byref(a), _raw_stream(q)), "packed_attention_bwd")
+            lib = _lib()
+            parts = lib.evlm_packed_attention_bwd_parts(C.byref(a))
+            if parts > 1:
+                ws = q.new_empty(parts * 2 * k.numel(), dtype=torch.float32)
+                a.workspace = ws.data_ptr()
+            L.check(lib.evlm_packed_attention_bwd(C.byref(a), _raw_stream(q)), "packed_attention_bwd")
         return dq, dk, dv, None, None, None, None, None
 
 
