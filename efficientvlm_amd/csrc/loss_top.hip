@@ -89,10 +89,18 @@ __device__ __forceinline__ int block_count(int v, int* red) {
 // One sweep finds every thread's own maximum; the k-th largest of those maxima (its upper 16 bits: a bisection by one wave) is
 // a lower bound of the k-th largest element, and barely more than k elements reach it.  Those are collected and ranked by
 // counting, (value, lower class first) making every element distinct - the result does not depend on the order of collection.
-// Rows with long ties at the bound (more candidates than the list holds) get the exact bound by bisection over the row, first
-// of the value, then of the class among equals.
+// Rows with long ties at the bound (more candidates than the list holds) and rows with NaN or without a finite maximum get the
+// exact bound by bisection over the row, first of the value, then of the class among equals.
+// Bound by its vector instructions as much as by HBM: 8 elements cost 12 instructions for the maximum, 56 slots for the sum and
+// one compare against the bound (their maximum is kept).
 #define TOP_NT 512
 #define TOP_CAP 1024
+#define TOP_LOG2E 1.44269504088896341f
+__device__ __forceinline__ float max8(const float (&v)[8]) {
+  return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+}
+// exp((v - m) / T), c2 = log2e / T.  (The difference first: a maximum of the type's lowest value times log2e would be -inf.)
+__device__ __forceinline__ float exp_diff(float v, float m, float c2) { return __builtin_amdgcn_exp2f((v - m) * c2); }
 template <typename T, int NCH>
 __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict__ logits, int C, int64_t ld, int k, float inv_t,
                                                             float* __restrict__ values, int32_t* __restrict__ classes,
@@ -109,6 +117,7 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
   const int chunks = (C + 7) >> 3;
   // rows of up to NCH * 8 * TOP_NT elements stay in registers between the sweeps (NCH = 0: longer ones are read again)
   TopRaw8<T> keep[NCH > 0 ? NCH : 1];
+  float most[NCH > 0 ? NCH : 1];                             // maximum of each 8
   if constexpr (NCH > 0) {
 #pragma unroll
     for (int n = 0; n < NCH; ++n)
@@ -121,27 +130,22 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
       f(v, 8 * c);
     }
   };
-  auto sweep = [&](auto f) __attribute__((always_inline)) {
-    if constexpr (NCH > 0) {
-#pragma unroll
-      for (int n = 0; n < NCH; ++n)
-        if (tid + n * TOP_NT < chunks) {
-          float v[8];
-          keep[n].get(v);
-          f(v, 8 * (tid + n * TOP_NT));
-        }
-    } else {
-      again(f);
-    }
-  };
   float mx = -INFINITY;
-  bool nan = false, any = false;
-  sweep([&](const float (&v)[8], int) {
-    any = true;
+  if constexpr (NCH > 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { mx = fmaxf(mx, v[e]); nan |= v[e] != v[e]; }
-  });
-  tops[tid] = any ? (nan ? 0xFFFFFFFFu : order_key(mx)) : 0u;
+    for (int n = 0; n < NCH; ++n) {
+      most[n] = -INFINITY;
+      if (tid + n * TOP_NT < chunks) {
+        float v[8];
+        keep[n].get(v);
+        most[n] = max8(v);
+        mx = fmaxf(mx, most[n]);
+      }
+    }
+  } else {
+    again([&](const float (&v)[8], int) { mx = fmaxf(mx, max8(v)); });
+  }
+  tops[tid] = tid < chunks ? order_key(mx) : 0u;
   if (tid == 0) count = 0;
   const float M = block_max(mx, red);                        // (ends the hand-over of tops and count, too)
   if (tid < 64) {
@@ -157,29 +161,59 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
     }
     if (lane == 0) bound = b;
   }
+  // sum of exp((v - M) / T): NaN where the row holds one, or has no finite maximum
+  const float c2 = inv_t * TOP_LOG2E;
   float s = 0.f;
-  const float top = M * inv_t;
-  if (top != -INFINITY && top != INFINITY)
-    sweep([&](const float (&v)[8], int) {
+  auto add8 = [&](const float (&v)[8], int) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += __expf(fmaf(v[e], inv_t, -top));
-    });
-  const bool bad = block_count(nan ? 1 : 0, ired) != 0;
-  s = block_sum(s, red);
-  if (tid == 0) lse[r] = bad ? __builtin_nanf("") : ((top == -INFINITY || top == INFINITY) ? top : top + __logf(s));
-  const uint32_t b = bound;
-  sweep([&](const float (&v)[8], int i0) {
+    for (int e = 0; e < 8; ++e) s += exp_diff(v[e], M, c2);
+  };
+  if constexpr (NCH > 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t key = order_key(v[e]);
-      if (key >= b && i0 + e < C) {
-        const int at = atomicAdd(&count, 1);
-        if (at < TOP_CAP) list[at] = ((unsigned long long)key << 32) | (uint32_t)~(i0 + e);
+    for (int n = 0; n < NCH; ++n)
+      if (tid + n * TOP_NT < chunks) {
+        float v[8];
+        keep[n].get(v);
+        add8(v, 0);
       }
+  } else {
+    again(add8);
+  }
+  s = block_sum(s, red);
+  const bool regular = s < INFINITY;                         // (block-uniform; false for NaN)
+  if (regular) {
+    if (tid == 0) lse[r] = M * inv_t + logf(s);
+    const float b = key_value(max(bound, 0x00800000u));      // (the lowest finite value at least)
+    auto collect = [&](const float (&v)[8], int i0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v[e] >= b && i0 + e < C) {
+          const int at = atomicAdd(&count, 1);
+          if (at < TOP_CAP) list[at] = ((unsigned long long)order_key(v[e]) << 32) | (uint32_t)~(i0 + e);
+        }
+    };
+    if constexpr (NCH > 0) {
+#pragma unroll
+      for (int n = 0; n < NCH; ++n)
+        if (most[n] >= b) {
+          float v[8];
+          keep[n].get(v);
+          collect(v, 8 * (tid + n * TOP_NT));
+        }
+    } else {
+      again([&](const float (&v)[8], int i0) { if (max8(v) >= b) collect(v, i0); });
     }
-  });
+  } else {
+    int nan = 0;
+    again([&](const float (&v)[8], int) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) nan |= v[e] != v[e] ? 1 : 0;
+    });
+    const bool bad = block_count(nan, ired) != 0;
+    if (tid == 0) lse[r] = bad ? __builtin_nanf("") : M;
+  }
   __syncthreads();
-  int n = count;
+  int n = regular && count >= k ? count : TOP_CAP + 1;       // (fewer than k finite ones: -inf has to be chosen among, too)
   if (n > TOP_CAP) {                                         // (block-uniform)
     auto reach = [&](uint32_t lo) {                          // elements with a key >= lo
       int m = 0;
@@ -253,29 +287,29 @@ extern "C" int evlm_top_logits(int dtype, const void* logits, int R, int C, int6
 // ---------------------------------------------------------------------------------------------
 #define KDT_NT 512
 // stats of a row, kept for the backward pass
-enum { ST_MAX = 0, ST_SUM, ST_NORM, ST_MASS, ST_MAX_REST, ST_SUM_REST, ST_P_REST, ST_N };
+// (maximum and sum of the row; teacher's normaliser and mass; raw maximum and sum of what the sweep covered; rest's mass)
+enum { ST_MAX = 0, ST_SUM, ST_NORM, ST_MASS, ST_RAW_MAX, ST_SWEEP_SUM, ST_P_REST, ST_N };
 
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {
+__device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[w] = v;
-  __syncthreads();
-  double t = 0.0;
-  for (int i = 0; i < nw; ++i) t += red[i];
-  return t;
+  return v;
 }
-__device__ __forceinline__ float exp_from(float x, float m) { return m == -INFINITY ? 0.f : __expf(x - m); }   // exp(x - m), x <= m
+__device__ __forceinline__ double wave_max_f64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ float exp_from(float x, float m) { return x == -INFINITY ? 0.f : __expf(x - m); }   // exp(x - m), x <= m
 
-template <typename T, bool REST>
-__global__ __launch_bounds__(KDT_NT) void kd_top_fwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
+// NCH > 0: rows of up to NCH * 8 * KDT_NT elements are asked for before anything else and stay in registers
+template <typename T, bool REST, int NCH>
+__global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void kd_top_fwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, const float* __restrict__ lse_t,
                                                             int k, float inv_t, const float* __restrict__ roww,
                                                             float* __restrict__ stats, float* __restrict__ rowloss) {
   extern __shared__ uint32_t kept[];                         // REST: one bit per class
   __shared__ float red[16];
-  __shared__ double dred[16];
   __shared__ int cls[TOP_MAX_K];
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x;
@@ -287,29 +321,40 @@ __global__ __launch_bounds__(KDT_NT) void kd_top_fwd_kernel(const T* __restrict_
   }
   const T* x = s + r * ld;
   const int words = (C + 31) >> 5, chunks = (C + 7) >> 3;
+  TopRaw8<T> keep[NCH > 0 ? NCH : 1];
+  if constexpr (NCH > 0) {
+#pragma unroll
+    for (int n = 0; n < NCH; ++n)
+      if (tid + n * KDT_NT < chunks) raw8<T>(x, tid + n * KDT_NT, C, -INFINITY, keep[n]);
+  }
+  // kept entries belong to the first wave: lane l holds entries l, l + 64, ..
+  constexpr int NE = TOP_MAX_K / 64;
+  int ci[NE];
+  bool twice = false;                                        // this lane met a class that was marked already
+  if (tid < 64) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int j = tid + 64 * i;
+      ci[i] = j < k ? classes[r * k + j] : -1;
+      if (ci[i] < 0 || ci[i] >= C) ci[i] = -1;
+    }
+  }
   if constexpr (REST) {
     for (int i = tid; i < words; i += KDT_NT) kept[i] = 0u;
     __syncthreads();
-  }
-  // kept entries: thread j < k holds entry j
-  int ci = -1;
-  float z = -INFINITY, y = -INFINITY;
-  if (tid < k) {
-    ci = classes[r * k + tid];
-    if (ci < 0 || ci >= C) ci = -1;
-    cls[tid] = ci;
-    if (ci >= 0) {
-      z = values[r * k + tid] * inv_t;
-      y = to_f(x[ci]) * inv_t;
-      if constexpr (REST) atomicOr(&kept[ci >> 5], 1u << (ci & 31));
+    if (tid < 64) {
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        if (tid + 64 * i < k) cls[tid + 64 * i] = ci[i];
+        const uint32_t bit = 1u << (ci[i] & 31);
+        if (ci[i] >= 0) twice |= (atomicOr(&kept[ci[i] >> 5], bit) & bit) != 0;
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
-  // one sweep: running maximum and sum of the row (REST: of the classes that are not kept)
-  float m = -INFINITY, sum = 0.f;
-  for (int c = tid; c < chunks; c += KDT_NT) {
-    float v[8];
-    row8<T>(x, c, C, -INFINITY, v);
+  // maximum and sum of the row (REST: of the classes that are not kept), thread by thread
+  const float c2 = inv_t * TOP_LOG2E;
+  auto drop_kept = [&](float (&v)[8], int c) __attribute__((always_inline)) {
     if constexpr (REST) {
       const uint32_t bits = (kept[c >> 2] >> (8 * (c & 3))) & 0xFFu;
       if (bits) {
@@ -317,52 +362,123 @@ __global__ __launch_bounds__(KDT_NT) void kd_top_fwd_kernel(const T* __restrict_
         for (int e = 0; e < 8; ++e) v[e] = (bits >> e) & 1u ? -INFINITY : v[e];
       }
     }
-    float mx = v[0];
+  };
+  float m = -INFINITY, sum = 0.f;
+  if constexpr (NCH > 0) {
 #pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, v[e]);
-    mx *= inv_t;
-    if (mx > m) { sum *= exp_from(m, mx); m = mx; }
-    const float base = m == -INFINITY ? 0.f : m;
+    for (int n = 0; n < NCH; ++n) {
+      const int c = tid + n * KDT_NT;
+      if (c < chunks) {
+        float v[8];
+        keep[n].get(v);
+        if constexpr (REST) {
+          if ((kept[c >> 2] >> (8 * (c & 3))) & 0xFFu) {
+            drop_kept(v, c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += __expf(fmaf(v[e], inv_t, -base));
-  }
-  // (maximum, log of the sum relative to it): one number would lose the sum next to a maximum of the type's lowest value
-  const float m_sweep = block_max(m, red);
-  sum = block_sum(m == -INFINITY ? sum : sum * exp_from(m, m_sweep), red);    // (NaN where the row holds one, even if m is -inf)
-  float top = m_sweep, total = sum;
-  if constexpr (REST) {                                      // + the kept classes, each once
-    bool first = ci >= 0;
-    for (int j = 0; j < tid && j < k; ++j) first = first && cls[j] != ci;
-    top = block_max(fmaxf(first ? y : -INFINITY, m_sweep), red);
-    total = block_sum(first && top != -INFINITY ? expf(y - top) : 0.f, red) + sum * exp_from(m_sweep, top);
-  }
-  const float ls = logf(total), ls_sweep = logf(sum);
-  // teacher.  p_rest is what is left of 1, so p and its sum are formed in 64 bits: one of a few per thousand would keep half of
-  // its digits in 32
-  const float zm = block_max(z, red);
-  float norm, p_rest = 0.f, p = 0.f, mass;
-  if constexpr (REST) {
-    norm = lse_t[r];
-    const double pd = ci >= 0 && z != -INFINITY ? exp((double)z - (double)norm) : 0.0;
-    p = (float)pd;
-    const double kept_mass = block_sum_f64(pd, dred);
-    mass = (float)kept_mass;
-    p_rest = sum == 0.f ? 0.f : (float)fmax(0.0, 1.0 - kept_mass);              // (sum == 0: no class is left for the rest)
-    if (kept_mass != kept_mass) p_rest = mass;
+            for (int e = 0; e < 8; ++e) keep[n].set(e, from_f<T>(v[e]));
+          }
+        }
+        m = fmaxf(m, max8(v));
+      }
+    }
   } else {
-    const float zs = block_sum(ci >= 0 && z != -INFINITY ? expf(z - zm) : 0.f, red);
-    norm = zm == -INFINITY ? -INFINITY : zm + logf(zs);
-    p = ci >= 0 && z != -INFINITY ? expf(z - zm) / zs : 0.f;
-    mass = zm == -INFINITY ? 0.f : 1.0f;
-    if (zs != zs) mass = zs;
+    for (int c = tid; c < chunks; c += KDT_NT) {
+      float v[8];
+      row8<T>(x, c, C, -INFINITY, v);
+      drop_kept(v, c);
+      m = fmaxf(m, max8(v));
+    }
   }
-  float L = p == 0.f ? 0.f : p * ((z - norm) - ((y - top) - ls));
-  L = block_sum(L, red);
+  m = block_max(m, red);
+  const float base = m == -INFINITY ? 0.f : m;
+  if constexpr (NCH > 0) {
+#pragma unroll
+    for (int n = 0; n < NCH; ++n)
+      if (tid + n * KDT_NT < chunks) {
+        float v[8];
+        keep[n].get(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += exp_diff(v[e], base, c2);
+      }
+  } else {
+    for (int c = tid; c < chunks; c += KDT_NT) {
+      float v[8];
+      row8<T>(x, c, C, -INFINITY, v);
+      drop_kept(v, c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += exp_diff(v[e], base, c2);
+    }
+  }
+  float z[NE], y[NE];
+  if (tid < 64) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      z[i] = ci[i] >= 0 ? values[r * k + tid + 64 * i] : 0.f;
+      y[i] = ci[i] >= 0 ? to_f(x[ci[i]]) : 0.f;
+    }
+  }
+  sum = block_sum(sum, red);                                 // (NaN where the row holds one)
+  if (tid >= 64) return;                                     // the rest is the first wave's
+  // A student close to its teacher has a loss of a few per thousand, the difference of terms of size 1, and p_rest is what is left
+  // of 1: the k + 1 terms are formed in 64 bits (32 kept four digits of such a row's loss).
+  // (Maximum, sum relative to it): a log-sum-exp in one number would lose the sum next to a maximum of the type's lowest value.
+  const double t = (double)inv_t, m_sweep = (double)m * t;
+  double top = m_sweep, total = (double)sum;
+  double yd[NE], zd[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) { yd[i] = ci[i] >= 0 ? (double)y[i] * t : -INFINITY; zd[i] = ci[i] >= 0 ? (double)z[i] * t : -INFINITY; }
+  if constexpr (REST) {                                      // + the kept classes, each once
+    bool first[NE];
+    double sk = 0.0;
+    const bool dup = __any(twice);
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      first[i] = ci[i] >= 0;
+      if (64 * i < k && dup)
+        for (int e = 0; e < k; ++e) first[i] = first[i] && !(e < tid + 64 * i && cls[e] == ci[i]);
+      if (first[i]) top = fmax(top, yd[i]);
+    }
+    top = wave_max_f64(top);
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (64 * i < k && first[i] && top != -INFINITY) sk += exp(yd[i] - top);
+    total = wave_sum_f64(sk) + (m_sweep == -INFINITY ? (sum != sum ? (double)sum : 0.0) : (double)sum * exp(m_sweep - top));
+  }
+  const double ls = log(total);
+  double norm, mass, p_rest = 0.0, p[NE] = {};
+  if constexpr (REST) {
+    norm = (double)lse_t[r];
+    mass = 0.0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (64 * i < k && zd[i] != -INFINITY) { p[i] = exp(zd[i] - norm); mass += p[i]; }
+    mass = wave_sum_f64(mass);
+    p_rest = mass != mass ? mass : (sum == 0.f ? 0.0 : fmax(0.0, 1.0 - mass));   // (sum == 0: no class is left for the rest)
+  } else {
+    double zm = -INFINITY, zs = 0.0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) zm = fmax(zm, zd[i]);
+    zm = wave_max_f64(zm);
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (64 * i < k && zd[i] != -INFINITY) { p[i] = exp(zd[i] - zm); zs += p[i]; }
+    zs = wave_sum_f64(zs);
+    norm = zm == -INFINITY ? -INFINITY : zm + log(zs);
+    mass = zm == -INFINITY ? (zs != zs ? zs : 0.0) : (zs != zs ? zs : 1.0);
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (64 * i < k && p[i] != 0.0) p[i] /= zs;
+  }
+  double L = 0.0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+    if (64 * i < k && p[i] != 0.0) L += p[i] * ((zd[i] - norm) - ((yd[i] - top) - ls));
+  L = wave_sum_f64(L);
   if (tid == 0) {
-    if (REST && p_rest != 0.f) L += p_rest * (logf(p_rest) - ((m_sweep - top) + (ls_sweep - ls)));
-    rowloss[r] = w * L;
-    st[ST_MAX] = top; st[ST_SUM] = total; st[ST_NORM] = norm; st[ST_MASS] = mass + p_rest;
-    if constexpr (REST) { st[ST_MAX_REST] = m_sweep; st[ST_SUM_REST] = sum; st[ST_P_REST] = p_rest; }
+    if (REST && p_rest != 0.0) L += p_rest * (log(p_rest) - ((m_sweep - top) + (log((double)sum) - ls)));
+    rowloss[r] = w * (float)L;
+    st[ST_MAX] = (float)top; st[ST_SUM] = (float)total; st[ST_NORM] = (float)norm; st[ST_MASS] = (float)(mass + p_rest);
+    st[ST_RAW_MAX] = m; st[ST_SWEEP_SUM] = sum; st[ST_P_REST] = (float)p_rest;
   }
 }
 __global__ __launch_bounds__(256) void kd_top_sum_kernel(const float* __restrict__ rowloss, int R, float coef, float* __restrict__ loss) {
@@ -418,16 +534,15 @@ __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict_
     for (int j = 0; j < k; ++j) p += cls[j] == ci ? prob[j] : 0.f;
     mine = g * (mass * (expf(y - top) / total) - p) + before;
   }
-  // the others: f * exp(y - max)
-  const float ref = REST ? st[ST_MAX_REST] : top, ref_sum = REST ? st[ST_SUM_REST] : total;
-  const float share = REST ? mass * (exp_from(ref, top) * ref_sum / total) - st[ST_P_REST] : mass;
-  const float f = ref_sum == 0.f && REST ? 0.f : g * share / ref_sum;           // (no class is left: nothing is written that stays)
-  const float base = ref == -INFINITY && REST ? 0.f : ref;
+  // the others: f * exp((v - raw maximum) / T)
+  const float c2 = inv_t * TOP_LOG2E, raw = st[ST_RAW_MAX], sweep = st[ST_SWEEP_SUM], base = raw == -INFINITY ? 0.f : raw;
+  const float share = REST ? mass * (exp_from(raw * inv_t, top) * sweep / total) - st[ST_P_REST] : mass;
+  const float f = REST && sweep == 0.f ? 0.f : g * share / sweep;               // (no class is left: nothing is written that stays)
   for (int c = tid; c < dchunks; c += KDT_NT) {
     float v[8];
     row8<T>(x, c, C, -INFINITY, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < C ? f * __expf(fmaf(v[e], inv_t, -base)) : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < C ? f * exp_diff(v[e], base, c2) : 0.f;
     if (acc) {
       float o[8];
       load8<T>(d + 8 * (int64_t)c, o);
@@ -453,11 +568,12 @@ extern "C" int evlm_kl_top_fwd(int dtype, const void* s, int R, int C, int64_t l
   hipStream_t stream = (hipStream_t)stream_;
   if (int rc = kd_top_check("evlm_kl_top_fwd", R, C, ld, k, inv_t)) return rc;
   EVLM_REQUIRE(s && values && classes && stats && rowloss && loss, "evlm_kl_top_fwd: null tensor");
+  const size_t bits = (size_t)((C + 31) / 32) * 4;
+#define KDT_FWD(REST, NCH, LDS) hipLaunchKernelGGL((kd_top_fwd_kernel<T, REST, NCH>), dim3(R), dim3(KDT_NT), LDS, stream, (const T*)s, C, ld, values, classes, lse_t, k, inv_t, row_weight, stats, rowloss)
   EVLM_DISPATCH_DTYPE(dtype, "evlm_kl_top_fwd",
-    if (lse_t)
-      hipLaunchKernelGGL((kd_top_fwd_kernel<T, true>), dim3(R), dim3(KDT_NT), (size_t)((C + 31) / 32) * 4, stream, (const T*)s, C, ld, values, classes, lse_t, k, inv_t, row_weight, stats, rowloss);
-    else
-      hipLaunchKernelGGL((kd_top_fwd_kernel<T, false>), dim3(R), dim3(KDT_NT), 0, stream, (const T*)s, C, ld, values, classes, lse_t, k, inv_t, row_weight, stats, rowloss);)
+    if (C <= 8 * 8 * KDT_NT) { if (lse_t) KDT_FWD(true, 8, bits); else KDT_FWD(false, 8, 0); }
+    else { if (lse_t) KDT_FWD(true, 0, bits); else KDT_FWD(false, 0, 0); })
+#undef KDT_FWD
   EVLM_LAUNCH_CHECK("evlm_kl_top_fwd");
   hipLaunchKernelGGL(kd_top_sum_kernel, dim3(1), dim3(256), 0, stream, (const float*)rowloss, R, weight / (float)R, loss);
   EVLM_LAUNCH_CHECK("evlm_kl_top_fwd");

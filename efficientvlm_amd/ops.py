@@ -1494,6 +1494,16 @@ def cross_attention(q, kv, H, dh, scale, mask=None, gate=None, want_probs=True, 
 # ---------------------------------------------------------------------------------------------------
 # attention over packed sequences (no map, no padding)
 # ---------------------------------------------------------------------------------------------------
+def _first_derivative(backward):
+    """a backward pass that has no derivative of its own: one that is itself recorded (create_graph=True) is refused, where its
+    gradients would silently count as constants"""
+    def checked(ctx, *g):
+        if torch.is_grad_enabled():
+            raise RuntimeError(f"{backward.__qualname__}: no second derivative (create_graph=True)")
+        return backward(ctx, *g)
+    return checked
+
+
 def _on_device_of(t):
     """launches go to the device the tensors live on, whatever the current one is"""
     return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
@@ -1566,7 +1576,7 @@ class _PackedAttention(torch.autograd.Function):
         return O
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, dO):
         q, k, v, cu_q, cu_k, k_lens, O, lo, lse = ctx.saved_tensors
         scale, causal = ctx.meta
@@ -2634,7 +2644,7 @@ class _KLTop(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, g):
         s2, values, classes, weight, work = ctx.saved_tensors
         R, Cn, ld, k, inv_t, rest, shape = ctx.meta
@@ -2689,7 +2699,8 @@ def soft_cross_entropy_top(predicts, values, classes, lse=None, temperature=1.0,
     L.require_cuda(predicts)
     if classes.dtype == torch.int64:           # (a class that does not fit stays outside)
         classes = classes.clamp(-1, predicts.shape[-1]).to(torch.int32)
-    f32 = lambda t: None if t is None else t.detach().to(torch.float32).contiguous()
+    f32 = lambda t: (t if t is None or (t.dtype == torch.float32 and t.is_contiguous() and not t.requires_grad)
+                     else t.detach().to(torch.float32).contiguous())
     return _KLTop.apply(predicts, f32(values), classes.contiguous(), f32(lse), f32(row_weight), 1.0 / T)
 
 

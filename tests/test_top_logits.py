@@ -347,6 +347,14 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.gpu
+def test_no_second_derivative():
+    s, v, c, l = pair(3, 50, 4, F32)
+    a = s.detach().requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(ops.soft_cross_entropy_top(a, v, c, lse=l), a, create_graph=True)
+
+
+@pytest.mark.gpu
 def test_join_with_the_hard_label_loss():
     """logits that feed the hard-label and the distillation loss: one gradient buffer (join_grads), the sum of both"""
     R, C = 20, 1001
