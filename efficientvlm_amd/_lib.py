@@ -97,8 +97,7 @@ SIGNATURES = {
     "evlm_xattn_fused_fwd": [C.POINTER(XAttnFusedArgs), _vp],
     "evlm_packed_attention_fwd": [C.POINTER(PackedAttnArgs), _vp],
     "evlm_packed_attention_bwd": [C.POINTER(PackedAttnArgs), _vp],
-    "evlm_packed_attention_splits": [C.POINTER(PackedAttnArgs)],
-    "evlm_packed_attention_bwd_parts": [C.POINTER(PackedAttnArgs)],
+    "evlm_packed_attention_workspace": [C.POINTER(PackedAttnArgs), _i],
     "evlm_mse_fwd": [_i, _vp, _i, _vp, _i64, _f, _vp, _vp],
     "evlm_mse_bwd": [_i, _vp, _i, _vp, _i64, _f, _vp, _vp, _vp],
     "evlm_ce_fwd": [_i, _vp, _i, _i, _i, _vp, _i, _f, _vp, _vp, _vp, _vp],

@@ -32,12 +32,13 @@ struct PkArgs {
   const void *Q, *K, *V, *O, *dO;
   void *out, *out_lo, *dQ, *dK, *dV;
   const int32_t *cu_q, *cu_k, *k_lens;
-  float *lse, *delta, *part, *part_ml;
+  float *lse, *delta, *part;
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head, dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
   int Tq, Tk, S, H, G, dh;          // G = heads per key head
   int gp, chunks, units;            // heads packed into a row block, chunks of a group, chunks * key heads
   int per, tiles;                   // tokens (keys) of a block, grid tiles
-  int splits, causal;               // splits: forward, parts of the keys; backward, parts of the rows of a key block
+  int splits, causal;               // splits: parts of the rows of a key block (dK / dV)
+  int want;                         // chunks of keys aimed at for one chunk of heads (forward, few rows)
   unsigned inv_gp;                  // 2^16 / gp rounded up: r / gp = r * inv_gp >> 16 for r < 256
   float scale, c;                   // c = scale * log2e
 };
@@ -221,6 +222,55 @@ template <bool KEYS> __device__ __forceinline__ bool find_tile(const PkArgs& a, 
   }
   over = (int)(t - before);
   total = (int)before;
+  return false;
+}
+// Few rows, many keys: the keys of every (sequence, block of tokens) are cut into chunks of one length for all, so that blocks of equal
+// work fill the chip however different the sequences are.  The length follows from the sequences themselves: their keys
+// (once for each block of tokens) over the number of chunks that is wanted, a multiple of 32, at least PK_CHUNK.
+#define PK_CHUNK 256
+struct Chunk { Seq q; int tile, chunk, n, keys; int64_t first; };       // `first`: index of the tile's first chunk among all
+__device__ __forceinline__ int chunks_of(const PkArgs& a, const Seq& x, int keys) { return max(1, (x.klen + keys - 1) / keys); }
+// the chunk with index g (BY_TOKEN: the first chunk of the block that holds token g); false: there is none
+template <bool BY_TOKEN> __device__ __forceinline__ bool find_chunk(const PkArgs& a, int g, Chunk& c) {
+  const int lane = threadIdx.x & 63;
+  int64_t work = 0;
+  for (int s = lane; s < a.S; s += 64) {
+    const Seq x = load_seq(a, s);
+    work += (int64_t)((x.qlen + a.per - 1) / a.per) * x.klen;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
+  const int64_t even = ((work + a.want - 1) / a.want + 31) / 32 * 32;
+  const int keys = even < PK_CHUNK ? PK_CHUNK : (even > (1 << 30) ? 1 << 30 : (int)even);
+  int64_t before = 0;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    Seq x = {0, 0, 0, 0};
+    int64_t n = 0;
+    if (s0 + lane < a.S) {
+      x = load_seq(a, s0 + lane);
+      n = (int64_t)((x.qlen + a.per - 1) / a.per) * chunks_of(a, x, keys);
+    }
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    const unsigned long long hit = __ballot(BY_TOKEN ? (g >= x.qs && g - x.qs < x.qlen) : before + incl > g);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      const int64_t first = before + __shfl(incl - n, l, 64);
+      c.q = uniform(load_seq(a, s0 + l));
+      c.n = __builtin_amdgcn_readfirstlane(chunks_of(a, c.q, keys));
+      c.keys = __builtin_amdgcn_readfirstlane(keys);
+      const int64_t rest = BY_TOKEN ? (int64_t)((g - c.q.qs) / a.per) * c.n : g - first;
+      c.tile = __builtin_amdgcn_readfirstlane((int)(rest / c.n));
+      c.chunk = __builtin_amdgcn_readfirstlane((int)(rest % c.n));
+      c.first = first + rest - rest % c.n;
+      return true;
+    }
+    before += __shfl(incl, 63, 64);
+  }
   return false;
 }
 // rows outside all sequences ([0, first start), [last end, T)): zeros.  `per_row(row)` by every wave of the surplus blocks
@@ -423,35 +473,42 @@ __global__ __launch_bounds__(64 * NW, 2) void pk_fwd_rows_kernel(PkArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// forward, keys split over the waves (and over `splits` blocks): 32 rows of one (sequence, chunk of heads) - single tokens and very
-// short sequences, where there are too few rows to fill a block of waves but perhaps many keys.  Every wave walks its own
-// 32-key blocks through its own LDS tile (no barrier in the loop) and the waves' sums are joined at the end.
+// forward, keys split over the waves: 32 rows of one (sequence, chunk of heads) - single tokens and very short sequences, where
+// there are too few rows to fill a block of waves but perhaps many keys.  Every wave walks its own 32-key blocks through its own
+// LDS tile (no barrier in the loop) and the waves' sums are joined at the end.  CH: a block takes one chunk of the keys (find_chunk)
+// and leaves its part for pk_join_kernel, unless the chunk is all there is.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
+// part of chunk g, chunk of heads `unit`: 32 x dh context (not divided by the sum), then 32 x (maximum, sum)
+__device__ __forceinline__ float* part_of(const PkArgs& a, int64_t g, int unit) {
+  return a.part + (g * a.units + unit) * (32 * (a.dh + 2));
+}
+template <typename T, int D, int NW, bool CH>
+__global__ __launch_bounds__(64 * NW, CH && sizeof(T) == 2 ? 2 : 1) void pk_fwd_keys_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
   constexpr int WB = 2 * 32 * TL::RB > 32 * D * 4 ? 2 * 32 * TL::RB : 32 * D * 4;       // one wave's tiles, later its context
   __shared__ __attribute__((aligned(512))) char sm[NW * WB];
   __shared__ float sml[NW][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
-  const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
-  const int rest = blockIdx.x / a.units, split = rest % a.splits;
-  Seq q; int ti, over, total;
-  if (!find_tile<false>(a, rest / a.splits, q, ti, over, total)) {
-    if (split == 0 && a.splits == 1) fwd_outside<T>(a, h0, over, total);
-    return;
+  const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp, g = blockIdx.x / a.units;
+  Seq q; int ti;
+  Chunk c;
+  if constexpr (CH) {
+    if (!find_chunk<false>(a, g, c)) return;                 // (rows outside all sequences: pk_join_kernel)
+    q = c.q; ti = c.tile;
+  } else {
+    int over, total;
+    if (!find_tile<false>(a, g, q, ti, over, total)) { fwd_outside<T>(a, h0, over, total); return; }
   }
   const int r = lane & 31, tok0 = ti * a.per, tok = tok0 + r / a.gp, h = h0 + r % a.gp;
   const bool valid = r < a.per * a.gp && tok < q.qlen;
   const int vis = valid ? vis_of(a, q, tok) : 0;
   const int last = min(tok0 + a.per, q.qlen) - 1;
   const int nk = vis_of(a, q, last), w_min = vis_of(a, q, tok0);
-  // this block's share of the keys: whole 32-key blocks, evenly
-  const int nb = (nk + 31) / 32, b0 = (int)((int64_t)nb * split / a.splits), b1 = (int)((int64_t)nb * (split + 1) / a.splits);
+  const int nb = (nk + 31) / 32, b0 = CH ? c.chunk * (c.keys / 32) : 0, b1 = CH ? min(nb, b0 + c.keys / 32) : nb;   // 32-key blocks
   char* Ks = sm + wave * WB;
   char* Vs = Ks + 32 * TL::RB;
   typename TL::frag qf[TL::NS];
@@ -475,6 +532,7 @@ __global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
     attend<T, D, 1>(Ks, Vs, kb * 32, vis, kb * 32 + 32 > w_min, qf, a.c, m, l, o, lane);
   }
   l += __shfl_xor(l, 32, 64);
+  const int64_t t = q.qs + tok;
   if constexpr (NW > 1) {
     // join the waves: wave w sums the row block's columns d = w * D / NW .. of every wave, rescaled to the common maximum
     wave_lds_fence();
@@ -495,10 +553,10 @@ __global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
       f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - M) * a.c);
       L += sml[w][1][r] * f[w];
     }
-    m = M; l = L;
     if (!valid) return;
-    const int64_t t = q.qs + tok;
+    const bool whole = !CH || c.n == 1;
     const float inv = vis > 0 ? 1.0f / L : 0.f;
+    float* part = CH ? part_of(a, c.first + c.chunk, unit) : nullptr;
     // thread -> (row r, 4 consecutive d): the 2 NW half-waves take them in turn
     for (int d = (wave * 2 + hh) * 4; d < a.dh; d += NW * 8) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -506,8 +564,8 @@ __global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
       for (int w = 0; w < NW; ++w)
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = fmaf(((float*)(sm + w * WB))[(d + j) * 32 + r], f[w], v[j]);
-      if (a.splits > 1) {
-        Vec4<float>::store(a.part + (((int64_t)split * a.H + h) * a.Tq + t) * a.dh + d, v);
+      if (!whole) {
+        Vec4<float>::store(part + r * a.dh + d, v);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] *= inv;
@@ -521,16 +579,14 @@ __global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
       }
     }
     if (wave == 0 && hh == 0) {
-      if (a.splits > 1) {
-        float* ml = a.part_ml + (((int64_t)split * a.H + h) * a.Tq + t) * 2;
-        ml[0] = m; ml[1] = l;
+      if (!whole) {
+        part[32 * a.dh + 2 * r] = M; part[32 * a.dh + 2 * r + 1] = L;
       } else if (a.lse) {
-        a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(m, a.c, __builtin_amdgcn_logf(l)) : INFINITY;
+        a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(M, a.c, __builtin_amdgcn_logf(L)) : INFINITY;
       }
     }
   } else {
     if (!valid) return;
-    const int64_t t = q.qs + tok;
     const float inv = vis > 0 ? 1.0f / l : 0.f;
     store_cols<T, D>((T*)a.out + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
     if (sizeof(T) == 2 && a.out_lo) store_rest<T, D>((T*)a.out_lo + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
@@ -538,35 +594,51 @@ __global__ __launch_bounds__(64 * NW, 1) void pk_fwd_keys_kernel(PkArgs a) {
   }
 }
 
-// join of the key splits: one wave per (token, head); a token outside all sequences has no parts and is zero
+// join of the chunks: one wave per (token, head), lanes over the head dim.  Rows of one chunk are done; a token outside all sequences
+// is zero.  The parts' maxima and sums are read 64 chunks at a time, the parts themselves a few at once
 template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkArgs a) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)a.Tq * a.H) return;
   const int lane = threadIdx.x & 63;
-  const int64_t t = row / a.H;
-  const int h = (int)(row % a.H);
-  const bool inside = a.S > 0 && t >= a.cu_q[0] && t < a.cu_q[a.S];
-  float M = -INFINITY;
-  if (inside)
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[(((int64_t)s * a.H + h) * a.Tq + t) * 2]);
-  float L = 0.f, v0 = 0.f, v1 = 0.f;
-  if (M != -INFINITY)
-    for (int s = 0; s < a.splits; ++s) {
-      const int64_t at = ((int64_t)s * a.H + h) * a.Tq + t;
-      const float ms = a.part_ml[at * 2];
-      if (ms == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f((ms - M) * a.c);
-      L = fmaf(a.part_ml[at * 2 + 1], f, L);
-      if (lane < a.dh) v0 = fmaf(a.part[at * a.dh + lane], f, v0);
-      if (lane + 64 < a.dh) v1 = fmaf(a.part[at * a.dh + lane + 64], f, v1);
+  const int t = __builtin_amdgcn_readfirstlane((int)(row / a.H)), h = __builtin_amdgcn_readfirstlane((int)(row % a.H));
+  Chunk c;
+  const bool inside = find_chunk<true>(a, t, c);
+  if (inside && c.n == 1) return;
+  T* o = (T*)a.out + ((int64_t)t * a.H + h) * a.dh;
+  float M = -INFINITY, L = 0.f, v0 = 0.f, v1 = 0.f;
+  if (inside) {
+    const int unit = h / a.gp, r = (t - c.q.qs - c.tile * a.per) * a.gp + h % a.gp;      // (heads of a unit are consecutive)
+    const int n = (int)min((int64_t)c.n, a.tiles - c.first);                             // (never past the workspace)
+    for (int i = lane; i < n; i += 64) M = fmaxf(M, part_of(a, c.first + i, unit)[32 * a.dh + 2 * r]);
+    M = wave_max(M);
+    if (M != -INFINITY) {
+      for (int i0 = 0; i0 < n; i0 += 64) {
+        float f = 0.f;
+        if (i0 + lane < n) {
+          const float* ml = part_of(a, c.first + i0 + lane, unit) + 32 * a.dh + 2 * r;
+          f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[0] - M) * a.c);
+          L = fmaf(ml[1], f, L);
+        }
+        const int e = min(64, n - i0);
+        const float* p = part_of(a, c.first + i0, unit) + r * a.dh;
+        const int64_t next = (int64_t)a.units * (32 * (a.dh + 2));
+        const int d0 = min(lane, a.dh - 1), d1 = min(lane + 64, a.dh - 1);
+#pragma unroll 8
+        for (int i = 0; i < e; ++i) {
+          const float fi = __shfl(f, i, 64);
+          v0 = fmaf(p[i * next + d0], fi, v0);
+          v1 = fmaf(p[i * next + d1], fi, v1);
+        }
+      }
+      L = wave_sum(L);
     }
+  }
   const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-  T* o = (T*)a.out + (t * a.H + h) * a.dh;
   v0 *= inv; v1 *= inv;
   if (lane < a.dh) o[lane] = from_f<T>(v0);
   if (lane + 64 < a.dh) o[lane + 64] = from_f<T>(v1);
   if (sizeof(T) == 2 && a.out_lo) {
-    T* lo = (T*)a.out_lo + (t * a.H + h) * a.dh;
+    T* lo = (T*)a.out_lo + ((int64_t)t * a.H + h) * a.dh;
     if (lane < a.dh) lo[lane] = from_f<T>(v0 - to_f(from_f<T>(v0)));
     if (lane + 64 < a.dh) lo[lane + 64] = from_f<T>(v1 - to_f(from_f<T>(v1)));
   }
@@ -825,6 +897,9 @@ template <typename T> __global__ __launch_bounds__(256) void pk_bwd_join_kernel(
 // ---------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------
+#ifndef PK_BLOCKS
+#define PK_BLOCKS 1536
+#endif
 static int largest_divisor(int n, int most) {
   for (int d = n < most ? n : most; d > 1; --d)
     if (n % d == 0) return d;
@@ -834,13 +909,15 @@ static bool pk_few_rows(const evlm_packed_attn_args* x, int gp) {
   // rows of a sequence and chunk of heads, on average: one wave's worth -> keys are split over the waves instead of rows
   return (int64_t)x->Tq * gp <= (int64_t)48 * x->S;
 }
-static int pk_splits(const evlm_packed_attn_args* x, int gp) {
-  if (!pk_few_rows(x, gp) || x->Tq == 0 || x->S == 0) return 1;
-  const int64_t blocks = ((int64_t)x->Tq * gp / 32 + x->S) * (x->H / gp);
-  const int64_t keys = x->Tk / x->S;                     // per sequence, on average
-  int64_t n = 512 / (blocks < 1 ? 1 : blocks);
-  if (n > keys / 256) n = keys / 256;
-  return n < 1 ? 1 : (n > 64 ? 64 : (int)n);
+// chunks of keys aimed at for each chunk of heads; 0: every block of rows walks all its keys.  Worth it where a sequence has room for
+// more than two chunks and the rows alone are few blocks
+static int pk_want(const evlm_packed_attn_args* x, int gp) {
+  if (x->S == 0 || x->Tq == 0 || !pk_few_rows(x, gp) || (int64_t)x->Tk <= (int64_t)2 * PK_CHUNK * x->S) return 0;
+  const int64_t units = x->H / gp, rows = ((int64_t)x->Tq * gp / 32 + x->S) * units;
+  return rows >= 2048 ? 0 : (int)((PK_BLOCKS + units - 1) / units);
+}
+static int64_t pk_chunk_slots(const evlm_packed_attn_args* x, int gp) {     // an upper bound of the chunks, whatever the lengths
+  return pk_want(x, gp) + (int64_t)x->Tq / (32 / gp) + x->S;
 }
 // dK / dV: row groups of a block of 4 waves; it covers 128 / groups keys
 static constexpr int pk_row_groups(int bytes, int D) { return bytes == 4 ? 1 : (D == 64 ? 4 : 2); }
@@ -892,30 +969,32 @@ static int pk_grid(PkArgs& a, int64_t T, int per, int units, const char* name, u
   return 0;
 }
 
-extern "C" int evlm_packed_attention_splits(const evlm_packed_attn_args* x) {
-  if (!x || x->H <= 0 || x->Hkv <= 0 || x->H % x->Hkv) return 1;
-  return pk_splits(x, largest_divisor(x->H / x->Hkv, 32));
+extern "C" int evlm_packed_attention_workspace(const evlm_packed_attn_args* x, int backward) {
+  if (!x || pk_check(x, "evlm_packed_attention_workspace")) return 0;       // (the call itself refuses such arguments)
+  const int gp = largest_divisor(x->H / x->Hkv, 32);
+  if (backward) {
+    const int parts = pk_parts(x);
+    return parts > 1 ? (int)((int64_t)parts * 2 * x->Tk * x->Hkv * x->dh) : 0;
+  }
+  return pk_want(x, gp) ? (int)(pk_chunk_slots(x, gp) * (x->H / gp) * 32 * (x->dh + 2)) : 0;
 }
 
-extern "C" int evlm_packed_attention_bwd_parts(const evlm_packed_attn_args* x) {
-  if (!x || x->H <= 0 || x->Hkv <= 0 || x->H % x->Hkv) return 1;
-  return pk_parts(x);
-}
-
-template <typename T, int D> static int pk_fwd_launch(PkArgs& a, bool few, hipStream_t stream) {
+template <typename T, int D> static int pk_fwd_launch(PkArgs& a, bool few, int64_t slots, hipStream_t stream) {
   unsigned grid;
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  if (few) {
+  if (a.want) {
+    a.per = 32 / a.gp;
+    a.tiles = (int)slots;
+    hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 4, true>), dim3((unsigned)(slots * a.units)), dim3(256), 0, stream, a);
+    EVLM_LAUNCH_CHECK("evlm_packed_attention_fwd");
+    const int64_t rows = (int64_t)a.Tq * a.H;
+    hipLaunchKernelGGL((pk_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+  } else if (few) {
     if (int rc = pk_grid(a, a.Tq, 32 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
-    if (a.splits == 1 && a.S > 0 && a.Tk / a.S <= 64)
-      hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 1>), dim3(grid), dim3(64), 0, stream, a);
+    if (a.S > 0 && a.Tk / a.S <= 64)
+      hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 1, false>), dim3(grid), dim3(64), 0, stream, a);
     else
-      hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 4>), dim3(grid), dim3(256), 0, stream, a);
-    if (a.splits > 1) {
-      EVLM_LAUNCH_CHECK("evlm_packed_attention_fwd");
-      const int64_t rows = (int64_t)a.Tq * a.H;
-      hipLaunchKernelGGL((pk_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
-    }
+      hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 4, false>), dim3(grid), dim3(256), 0, stream, a);
   } else {
     if (int rc = pk_grid(a, a.Tq, 128 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
     hipLaunchKernelGGL((pk_fwd_rows_kernel<T, D, 4, BN>), dim3(grid), dim3(256), 0, stream, a);
@@ -935,13 +1014,13 @@ extern "C" int evlm_packed_attention_fwd(const evlm_packed_attn_args* x, void* s
   EVLM_REQUIRE(x->Q && x->O && (x->Tk == 0 || (x->K && x->V)), "evlm_packed_attention_fwd: null tensor");
   PkArgs a = pk_args(x);
   const bool few = x->S > 0 && pk_few_rows(x, a.gp);
-  a.splits = pk_splits(x, a.gp);
-  if (a.splits > 1) {
-    EVLM_REQUIRE(x->workspace, "evlm_packed_attention_fwd: %d key splits need a workspace", a.splits);
+  a.want = pk_want(x, a.gp);
+  const int64_t slots = a.want ? pk_chunk_slots(x, a.gp) : 0;
+  if (a.want) {
+    EVLM_REQUIRE(x->workspace, "evlm_packed_attention_fwd: this many keys for so few rows need a workspace");
     a.part = (float*)x->workspace;
-    a.part_ml = a.part + (int64_t)a.splits * x->H * x->Tq * x->dh;
   }
-  return PK_DISPATCH(x, pk_fwd_launch)(a, few, (hipStream_t)stream_);
+  return PK_DISPATCH(x, pk_fwd_launch)(a, few, slots, (hipStream_t)stream_);
 }
 
 template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, bool few_keys, int parts, hipStream_t stream) {

@@ -1565,9 +1565,9 @@ class _PackedAttention(torch.autograd.Function):
                 if q.dtype == torch.bfloat16:                   # (what rounding takes from O)
                     lo = torch.empty_like(O)
                     a.O_lo = lo.data_ptr()
-            splits = lib.evlm_packed_attention_splits(C.byref(a))
-            if splits > 1:
-                ws = q.new_empty(splits * H * Tq * (dh + 2), dtype=torch.float32)
+            n = lib.evlm_packed_attention_workspace(C.byref(a), 0)
+            if n:
+                ws = q.new_empty(n, dtype=torch.float32)
                 a.workspace = ws.data_ptr()
             L.check(lib.evlm_packed_attention_fwd(C.byref(a), _raw_stream(q)), "packed_attention_fwd")
         if need:
@@ -1594,9 +1594,9 @@ class _PackedAttention(torch.autograd.Function):
             a.dq_tok, a.dk_tok, a.dv_tok = H * dh, k.shape[1] * dh, k.shape[1] * dh
             a.dq_head = a.dk_head = a.dv_head = dh
             lib = _lib()
-            parts = lib.evlm_packed_attention_bwd_parts(C.byref(a))
-            if parts > 1:
-                ws = q.new_empty(parts * 2 * k.numel(), dtype=torch.float32)
+            n = lib.evlm_packed_attention_workspace(C.byref(a), 1)
+            if n:
+                ws = q.new_empty(n, dtype=torch.float32)
                 a.workspace = ws.data_ptr()
             L.check(lib.evlm_packed_attention_bwd(C.byref(a), _raw_stream(q)), "packed_attention_bwd")
         return dq, dk, dv, None, None, None, None, None

@@ -299,8 +299,7 @@ int evlm_copy_few(const void* const* src, void* const* dst, const int64_t* nbyte
  *   causal: query i of n sees keys j < m - n + i + 1 of m (the last query sees all).  A row that sees no key, and a row outside
  *   all sequences, has O = 0; so have the gradients of keys that no row sees.
  *   lse [H, Tq] f32 (forward: written if given; backward: as the forward wrote it).  delta [H, Tq] f32: backward scratch.
- *   workspace (uninitialised): forward, only if n = evlm_packed_attention_splits() > 1: n * H * Tq * (dh + 2) floats; backward,
- *   only if n = evlm_packed_attention_bwd_parts() > 1: n * 2 * Tk * Hkv * dh floats.
+ *   workspace: evlm_packed_attention_workspace() floats, uninitialised, for one call at a time.
  * The decoder side of the reference pads its answers to the longest (eff_bert.py:317-355 over [B, L] rows, the causal mask of
  * :975-996); packed rows do the same arithmetic without the padding.
  * ---------------------------------------------------------------------------------------------- */
@@ -324,10 +323,9 @@ typedef struct {
 } evlm_packed_attn_args;
 int evlm_packed_attention_fwd(const evlm_packed_attn_args* a, void* stream);
 int evlm_packed_attention_bwd(const evlm_packed_attn_args* a, void* stream);
-/* number of parts the forward cuts the keys into, and the backward the rows of a block of keys (rules on Tq, Tk, S, H, Hkv);
- * 1: no workspace */
-int evlm_packed_attention_splits(const evlm_packed_attn_args* a);
-int evlm_packed_attention_bwd_parts(const evlm_packed_attn_args* a);
+/* floats of workspace a forward / backward call takes (a rule on Tq, Tk, S, H, Hkv, dh, dtype): parts of long key ranges
+ * that few rows attend to, parts of the rows of few blocks of keys; 0: none */
+int evlm_packed_attention_workspace(const evlm_packed_attn_args* a, int backward);
 
 /* ------------------------------------------------------------------------------------------------
  * Fused cross-attention FORWARD: K/V projection of the image tokens + Q K^T + softmax + P V (+ the map) in one launch.
