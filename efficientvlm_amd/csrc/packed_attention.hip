@@ -57,9 +57,15 @@ __device__ __forceinline__ f32x16 mma(const f32x4& a, const f32x4& b, f32x16 c) 
   return c;
 }
 
-// LDS addresses as numbers: all pieces of a row, and all column blocks of 4 rows, lie at base ^ (constant)
+// LDS addresses as numbers: all pieces of a row, and all column blocks of 4 rows, lie at base ^ (constant).  The compiler keeps a
+// register for each of them; a LEAN kernel makes the base opaque where it is used, so that the few exclusive-ors are done again
+// in every iteration.  (dK / dV at head dim 128 fits two waves a SIMD only so; the forward pass lost 7 % by it.)
 typedef __attribute__((address_space(3))) const char* lds_ptr;
 __device__ __forceinline__ uint32_t lds_of(const char* p) { return (uint32_t)(uintptr_t)(lds_ptr)p; }
+template <bool LEAN> __device__ __forceinline__ uint32_t base_of(uint32_t x) {
+  if (LEAN) asm volatile("" : "+v"(x));
+  return x;
+}
 template <typename F> __device__ __forceinline__ F lds_read(uint32_t at) { return *(__attribute__((address_space(3))) const F*)(uintptr_t)at; }
 
 // Row-major LDS tile [rows][D], 16-byte pieces of a row permuted so that neither the row reads (16 rows, one piece each) nor
@@ -82,11 +88,19 @@ template <typename T, int D> struct Tile {
       if (row && e < dh) f[s] = *reinterpret_cast<const frag*>(row + e);
     }
   }
-  static __device__ __forceinline__ f32x16 row_mm(const char* tile, int r0, const frag (&b)[NS], int lane) {
+  template <bool LEAN = false> static __device__ __forceinline__ f32x16 row_mm(const char* tile, int r0, const frag (&b)[NS], int lane) {
     f32x16 acc = {};
-    const uint32_t base = lds_of(tile) + at(r0 + (lane & 31), lane >> 5);
+    const uint32_t base = base_of<LEAN>(lds_of(tile) + at(r0 + (lane & 31), lane >> 5));
 #pragma unroll
     for (int s = 0; s < NS; ++s) acc = mma(lds_read<frag>(base ^ (32 * s)), b[s], acc);
+    return acc;
+  }
+  // columns from LDS as well (32 rows of another tile)
+  static __device__ __forceinline__ f32x16 row_mm(const char* tile, int r0, const char* cols, int c0, int lane) {
+    f32x16 acc = {};
+    const uint32_t rows = base_of<true>(lds_of(tile) + at(r0 + (lane & 31), lane >> 5)), col = base_of<true>(lds_of(cols) + at(c0 + (lane & 31), lane >> 5));
+#pragma unroll
+    for (int s = 0; s < NS; ++s) acc = mma(lds_read<frag>(rows ^ (32 * s)), lds_read<frag>(col ^ (32 * s)), acc);
     return acc;
   }
   // NB blocks of 32 rows against the same columns
@@ -104,10 +118,10 @@ template <typename T, int D> struct Tile {
 // acc[d][c] += sum_r tile[r][d] p[r][c]
 // bf16: register i of C holds tile row 8 (i >> 2) + 4 (lane >> 5) + (i & 3); registers 8kk .. 8kk + 7 are the B operand of k-step
 // kk, and the A operand takes its 8 rows in that order: two transposing reads of 4 rows x 16 columns each
-template <int D> __device__ __forceinline__ void col_mm(const bf16*, const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+template <int D, bool LEAN = false> __device__ __forceinline__ void col_mm(const bf16*, const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
   typedef Tile<bf16, D> TL;
   const int hh = lane >> 5, w = lane & 15, sub = (lane >> 4) & 1;
-  const uint32_t base = lds_of(tile) + TL::at(r0 + 4 * hh + (w >> 2), sub * 2 + ((w & 3) >> 1)) + (w & 1) * 8;
+  const uint32_t base = base_of<LEAN>(lds_of(tile) + TL::at(r0 + 4 * hh + (w >> 2), sub * 2 + ((w & 3) >> 1)) + (w & 1) * 8);
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
     bf16x8 b;
@@ -126,7 +140,7 @@ template <int D> __device__ __forceinline__ void col_mm(const bf16*, const char*
     }
   }
 }
-template <int D> __device__ __forceinline__ void col_mm(const float*, const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
+template <int D, bool LEAN = false> __device__ __forceinline__ void col_mm(const float*, const char* tile, int r0, const f32x16& p, f32x16 (&acc)[D / 32], int lane) {
   const int hh = lane >> 5, w = lane & 31;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -725,19 +739,21 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
 
 // ---------------------------------------------------------------------------------------------
 // backward, dK / dV.  A wave holds 32 keys as columns; the NW waves are NW / RG groups of keys x RG groups of rows, whose sums are
-// joined at the end.  The rows of every head of the group stream through LDS, RG * RB * 32 at a time: a wave takes RB blocks of 32
-// between two barriers, so that the products of one and the exponentials of the other can overlap.  `splits` blocks share the
-// rows of a key block and leave f32 parts (joined by pk_bwd_join_kernel) where there are few key blocks.
+// joined at the end.  The rows of every head of the group stream through LDS, RG * 32 at a time.  `splits` blocks share the rows of
+// a key block and leave f32 parts (joined by pk_bwd_join_kernel) where there are few key blocks.
+// VL: V is read from LDS as well.  At head dim 128 the two accumulators take 128 registers, K and V as columns 64, two blocks of
+// scores 32: without V two waves fit a SIMD, and they hide what one wave with all of it in registers (512) had to wait for.
+// One register too many is worse than either: a spill's reload waits for the loads of the next rows.
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int NW, int RG, int RB>
-__global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 ? 2 : 1) void pk_bwd_dkv_kernel(PkArgs a) {
+template <typename T, int D, int NW, int RG, bool VL>
+__global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || VL ? 2 : 1) void pk_bwd_dkv_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
-  constexpr int BR = 32 * RG * RB, KG = NW / RG, JOIN = KG * (RG - 1) * 32 * D * 4;
-  constexpr int SM = 2 * BR * TL::RB > JOIN ? 2 * BR * TL::RB : JOIN;
+  constexpr int BR = 32 * RG, KG = NW / RG, JOIN = KG * (RG - 1) * 32 * D * 4;
+  constexpr int VB = VL ? KG * 32 * TL::RB : 0, SM = VB + 2 * BR * TL::RB > JOIN ? VB + 2 * BR * TL::RB : JOIN;
   __shared__ __attribute__((aligned(512))) char sm[SM];
   __shared__ __attribute__((aligned(16))) float Ls[BR], Ds[BR];
   __shared__ __attribute__((aligned(16))) int Vis[BR];
-  char *Qs = sm, *Os = sm + BR * TL::RB;
+  char *Vs = sm, *Qs = sm + VB, *Os = Qs + BR * TL::RB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, kg = wave / RG, rg = wave % RG;
   const int nkh = a.H / a.G, kh = blockIdx.x % nkh;
   const int rest = blockIdx.x / nkh, part = rest % a.splits;
@@ -754,6 +770,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 ? 2 : 1) void pk_bwd_
   typename TL::frag kf[TL::NS], vf[TL::NS];
   TL::load_cols(key < q.klen ? (const T*)a.K + (q.ks + (int64_t)key) * a.k_tok + kh * a.k_head : nullptr, a.dh, hh, kf);
   TL::load_cols(key < q.klen ? (const T*)a.V + (q.ks + (int64_t)key) * a.v_tok + kh * a.v_head : nullptr, a.dh, hh, vf);
+  if constexpr (VL) {                                        // (the row groups of a key group write the same)
+#pragma unroll
+    for (int s = 0; s < TL::NS; ++s) *reinterpret_cast<typename TL::frag*>(Vs + TL::at(key - k0, 2 * s + hh)) = vf[s];
+  }
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
   const int btok = (int)(BR * a.inv_gp >> 16), used = btok * a.gp;
   // row blocks: the tokens from the first that sees key k0, for one chunk of heads after the other
@@ -791,39 +811,31 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 ? 2 : 1) void pk_bwd_
     if (b + 1 < b1) load(ch, tok0);
     // this wave's rows: tokens t_lo .. t_hi of the block.  Nothing to do if the last of them sees none of the wave's keys; masked
     // if the first does not see all of them (columns behind the last key are not stored)
-    const int r_lo = 32 * RB * rg;
-    const int t_lo = now + (int)(r_lo * a.inv_gp >> 16), t_hi = min(now + (int)((r_lo + 32 * RB - 1) * a.inv_gp >> 16), q.qlen - 1);
+    const int r_lo = 32 * rg;
+    const int t_lo = now + (int)(r_lo * a.inv_gp >> 16), t_hi = min(now + (int)((r_lo + 31) * a.inv_gp >> 16), q.qlen - 1);
     if (t_lo >= q.qlen || vis_of(a, q, t_hi) <= w0) continue;
     const bool mask = a.causal && vis_of(a, q, t_lo) < w0 + 32;
-    f32x16 p[RB], ds[RB];
-#pragma unroll
-    for (int n = 0; n < RB; ++n) {
-      p[n] = TL::row_mm(Qs, r_lo + 32 * n, kf, lane);
-      ds[n] = TL::row_mm(Os, r_lo + 32 * n, vf, lane);
-    }
+    f32x16 p = TL::template row_mm<VL>(Qs, r_lo, kf, lane), ds;
+    if constexpr (VL) ds = TL::row_mm(Os, r_lo, Vs, w0 - k0, lane);
+    else ds = TL::row_mm(Os, r_lo, vf, lane);
     if (mask) {
 #pragma unroll
-      for (int n = 0; n < RB; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[n][i] = key < Vis[r_lo + 32 * n + c_row(i, hh)] ? p[n][i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) p[i] = key < Vis[r_lo + c_row(i, hh)] ? p[i] : -INFINITY;
     }
 #pragma unroll
-    for (int n = 0; n < RB; ++n) {
+    for (int j = 0; j < 4; ++j) {
+      const int r0 = r_lo + 8 * j + 4 * hh;
+      const f32x4 l4 = *reinterpret_cast<const f32x4*>(Ls + r0), d4 = *reinterpret_cast<const f32x4*>(Ds + r0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r0 = r_lo + 32 * n + 8 * j + 4 * hh;
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(Ls + r0), d4 = *reinterpret_cast<const f32x4*>(Ds + r0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * j + e;
-          const float x = __builtin_amdgcn_exp2f(fmaf(p[n][i], a.c, -l4[e]));
-          ds[n][i] = x * (ds[n][i] - d4[e]);
-          p[n][i] = x;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * j + e;
+        const float x = __builtin_amdgcn_exp2f(fmaf(p[i], a.c, -l4[e]));
+        ds[i] = x * (ds[i] - d4[e]);
+        p[i] = x;
       }
-      col_mm<D>((const T*)nullptr, Os, r_lo + 32 * n, p[n], dv, lane);
-      col_mm<D>((const T*)nullptr, Qs, r_lo + 32 * n, ds[n], dk, lane);
     }
+    col_mm<D, VL>((const T*)nullptr, Os, r_lo, p, dv, lane);
+    col_mm<D, VL>((const T*)nullptr, Qs, r_lo, ds, dk, lane);
   }
   if constexpr (RG > 1) {                                     // join the row groups, dK first, then dV
     auto join = [&](f32x16 (&acc)[D / 32]) {
@@ -865,12 +877,14 @@ template <typename T> __global__ __launch_bounds__(256) void pk_bwd_join_kernel(
   const int64_t key = blockIdx.x;
   const int nkh = a.H / a.G, row = nkh * a.dh;
   // last sequence that starts at or before this key
-  int lo = 0, hi = a.S;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_k[mid] <= key) lo = mid + 1; else hi = mid;
+  int s = -1;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    const int i = s0 + (threadIdx.x & 63);
+    const int n = __popcll(__ballot(i < a.S && a.cu_k[i] <= key));
+    s += n;
+    if (n < 64) break;
   }
-  const int s = lo - 1;
+  s = __builtin_amdgcn_readfirstlane(s);
   bool inside = false, room = false;
   if (s >= 0) {
     const Seq q = load_seq(a, s);
@@ -919,17 +933,24 @@ static int pk_want(const evlm_packed_attn_args* x, int gp) {
 static int64_t pk_chunk_slots(const evlm_packed_attn_args* x, int gp) {     // an upper bound of the chunks, whatever the lengths
   return pk_want(x, gp) + (int64_t)x->Tq / (32 / gp) + x->S;
 }
-// dK / dV: row groups of a block of 4 waves; it covers 128 / groups keys
-static constexpr int pk_row_groups(int bytes, int D) { return bytes == 4 ? 1 : (D == 64 ? 4 : 2); }
+// dK / dV, the shape of a block: waves, groups of rows among them; the other factor are groups of 32 keys
+template <typename T, int D> struct DkvShape { static constexpr int NW = 4, RG = sizeof(T) == 4 ? 1 : 4, KEYS = 32 * NW / RG; static constexpr bool VL = false; };
+template <> struct DkvShape<bf16, 128> { static constexpr int NW = 8, RG = 1, KEYS = 256; static constexpr bool VL = true; };
 static bool pk_few_keys(const evlm_packed_attn_args* x) { return (int64_t)x->Tk <= (int64_t)48 * x->S; }
-// ... parts of the rows of a key block, where there are too few key blocks for the chip; each part still has some hundred rows
-static int pk_parts(const evlm_packed_attn_args* x) {
-  if (x->S == 0 || x->Tk == 0 || pk_few_keys(x)) return 1;
-  const int keys = 128 / pk_row_groups(x->dtype == EVLM_BF16 ? 2 : 4, x->dh <= 64 ? 64 : 128);
-  const int64_t blocks = ((int64_t)x->Tk / keys + x->S) * x->Hkv, rows = (int64_t)x->Tq * (x->H / x->Hkv) / x->S;
-  int64_t n = (256 + blocks - 1) / blocks;
+// ... parts of the rows of a key block, where there are too few key blocks for the chip; each part still has some hundred rows.
+// 256-key blocks are long and (causal) of very different lengths: they want three a CU (5 x 176 blocks of the documents' 10 156
+// keys and 4 key heads: 607 us backward; 3 x 176: 670; undivided 64-key blocks of 4 waves: 715), shorter ones just the CUs filled
+template <typename T, int D> static int pk_parts_of(const evlm_packed_attn_args* x) {
+  typedef DkvShape<T, D> SH;
+  const int64_t blocks = ((int64_t)x->Tk / SH::KEYS + x->S) * x->Hkv, rows = (int64_t)x->Tq * (x->H / x->Hkv) / x->S;
+  int64_t n = ((SH::KEYS == 256 ? 768 : 256) + blocks - 1) / blocks;
   if (n > rows / 512) n = rows / 512;
   return n < 1 ? 1 : (n > 8 ? 8 : (int)n);
+}
+static int pk_parts(const evlm_packed_attn_args* x) {
+  if (x->S == 0 || x->Tk == 0 || pk_few_keys(x)) return 1;
+  return x->dtype == EVLM_BF16 ? (x->dh <= 64 ? pk_parts_of<bf16, 64>(x) : pk_parts_of<bf16, 128>(x))
+                               : (x->dh <= 64 ? pk_parts_of<float, 64>(x) : pk_parts_of<float, 128>(x));
 }
 static int pk_check(const evlm_packed_attn_args* x, const char* name) {
   EVLM_REQUIRE(x->dtype == EVLM_F32 || x->dtype == EVLM_BF16, "%s: bad dtype %d", name, x->dtype);
@@ -1042,11 +1063,11 @@ template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, bool 
     a.splits = parts;
     if (few_keys) {
       if (int rc = pk_grid(a, a.Tk, 32, nkh, name, &grid)) return rc;
-      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 1, 1, 1>), dim3(grid), dim3(64), 0, stream, a);
+      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 1, 1, false>), dim3(grid), dim3(64), 0, stream, a);
     } else {
-      constexpr int RG = pk_row_groups((int)sizeof(T), D);
-      if (int rc = pk_grid(a, a.Tk, 128 / RG, nkh, name, &grid)) return rc;
-      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 4, RG, (sizeof(T) == 2 && D == 128 ? 2 : 1)>), dim3(grid), dim3(256), 0, stream, a);
+      typedef DkvShape<T, D> SH;
+      if (int rc = pk_grid(a, a.Tk, SH::KEYS, nkh, name, &grid)) return rc;
+      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, SH::NW, SH::RG, SH::VL>), dim3(grid), dim3(64 * SH::NW), 0, stream, a);
     }
     if (a.splits > 1) {
       EVLM_LAUNCH_CHECK(name);
