@@ -637,7 +637,6 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
         const float* p = part_of(a, c.first + i0, unit) + r * a.dh;
         const int64_t next = (int64_t)a.units * (32 * (a.dh + 2));
         const int d0 = min(lane, a.dh - 1), d1 = min(lane + 64, a.dh - 1);
-#pragma unroll 8
         for (int i = 0; i < e; ++i) {
           const float fi = __shfl(f, i, 64);
           v0 = fmaf(p[i * next + d0], fi, v0);
@@ -746,7 +745,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
 // One register too many is worse than either: a spill's reload waits for the loads of the next rows.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int RG, bool VL>
-__global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || VL ? 2 : 1) void pk_bwd_dkv_kernel(PkArgs a) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) void pk_bwd_dkv_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
   constexpr int BR = 32 * RG, KG = NW / RG, JOIN = KG * (RG - 1) * 32 * D * 4;
   constexpr int VB = VL ? KG * 32 * TL::RB : 0, SM = VB + 2 * BR * TL::RB > JOIN ? VB + 2 * BR * TL::RB : JOIN;
@@ -911,9 +910,7 @@ template <typename T> __global__ __launch_bounds__(256) void pk_bwd_join_kernel(
 // ---------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------
-#ifndef PK_BLOCKS
 #define PK_BLOCKS 1536
-#endif
 static int largest_divisor(int n, int most) {
   for (int d = n < most ? n : most; d > 1; --d)
     if (n % d == 0) return d;
@@ -934,21 +931,29 @@ static int64_t pk_chunk_slots(const evlm_packed_attn_args* x, int gp) {     // a
   return pk_want(x, gp) + (int64_t)x->Tq / (32 / gp) + x->S;
 }
 // dK / dV, the shape of a block: waves, groups of rows among them; the other factor are groups of 32 keys
-template <typename T, int D> struct DkvShape { static constexpr int NW = 4, RG = sizeof(T) == 4 ? 1 : 4, KEYS = 32 * NW / RG; static constexpr bool VL = false; };
+template <typename T, int D> struct DkvShape { static constexpr int NW = 4, RG = sizeof(T) == 4 ? 1 : 4, KEYS = 32 * NW / RG; static constexpr bool VL = D > 64; };
 template <> struct DkvShape<bf16, 128> { static constexpr int NW = 8, RG = 1, KEYS = 256; static constexpr bool VL = true; };
-static bool pk_few_keys(const evlm_packed_attn_args* x) { return (int64_t)x->Tk <= (int64_t)48 * x->S; }
+// ... blocks of one wave, 32 keys, for short key ranges.  16 384 tokens, heads 8/8, backward in us, one wave against a full block:
+// bf16 dim 64, 24 keys a sequence 85 / 201, 72: 77 / 117, 150: 76 / 105, 250: 77 / 108 (heads 16/4: 150: 96 / 104, 250: 119 / 117);
+// bf16 dim 128, 24: 172 / 293, 44: 145 / 195 (100 keys, blocks of four waves that share 32 keys: 297 / 156).  f32 at dim 128 has
+// no such kernel: with all of K, V and both sums in one wave's registers it spilled (4096 tokens, heads 16/4, 44 keys: 311 / 234)
+template <typename T, int D> static bool pk_few_keys(int Tk, int S) {
+  if (D > 64 && sizeof(T) == 4) return false;
+  return (int64_t)Tk <= (int64_t)(D <= 64 ? 160 : 48) * S;
+}
 // ... parts of the rows of a key block, where there are too few key blocks for the chip; each part still has some hundred rows.
 // 256-key blocks are long and (causal) of very different lengths: they want three a CU (5 x 176 blocks of the documents' 10 156
 // keys and 4 key heads: 607 us backward; 3 x 176: 670; undivided 64-key blocks of 4 waves: 715), shorter ones just the CUs filled
 template <typename T, int D> static int pk_parts_of(const evlm_packed_attn_args* x) {
   typedef DkvShape<T, D> SH;
+  if (pk_few_keys<T, D>(x->Tk, x->S)) return 1;
   const int64_t blocks = ((int64_t)x->Tk / SH::KEYS + x->S) * x->Hkv, rows = (int64_t)x->Tq * (x->H / x->Hkv) / x->S;
   int64_t n = ((SH::KEYS == 256 ? 768 : 256) + blocks - 1) / blocks;
   if (n > rows / 512) n = rows / 512;
   return n < 1 ? 1 : (n > 8 ? 8 : (int)n);
 }
 static int pk_parts(const evlm_packed_attn_args* x) {
-  if (x->S == 0 || x->Tk == 0 || pk_few_keys(x)) return 1;
+  if (x->S == 0 || x->Tk == 0) return 1;
   return x->dtype == EVLM_BF16 ? (x->dh <= 64 ? pk_parts_of<bf16, 64>(x) : pk_parts_of<bf16, 128>(x))
                                : (x->dh <= 64 ? pk_parts_of<float, 64>(x) : pk_parts_of<float, 128>(x));
 }
@@ -1044,15 +1049,20 @@ extern "C" int evlm_packed_attention_fwd(const evlm_packed_attn_args* x, void* s
   return PK_DISPATCH(x, pk_fwd_launch)(a, few, slots, (hipStream_t)stream_);
 }
 
-template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, bool few_keys, int parts, hipStream_t stream) {
+template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, int parts, hipStream_t stream) {
   unsigned grid;
   constexpr int BN = sizeof(T) == 2 ? 64 : 32;
   const char* name = "evlm_packed_attention_bwd";
   const int nkh = a.H / a.G;
   if (a.Tq > 0) {
-    if (few) {
-      if (int rc = pk_grid(a, a.Tq, 32 / a.gp, a.units, name, &grid)) return rc;
-      hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 1, 32>), dim3(grid), dim3(64), 0, stream, a);
+    // one wave a block for few rows (16 384 tokens, heads 8/8, 24 a sequence, bf16 dim 128: backward 171 us, 224 with blocks of four),
+    // but not at dim 128 in f32, where it spilled (4096 tokens, heads 16/4, 24 a sequence: 267 us, 227 with blocks of four)
+    constexpr bool kOneWave = D <= 64 || sizeof(T) == 2;
+    if (few && kOneWave) {
+      if constexpr (kOneWave) {
+        if (int rc = pk_grid(a, a.Tq, 32 / a.gp, a.units, name, &grid)) return rc;
+        hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 1, 32>), dim3(grid), dim3(64), 0, stream, a);
+      }
     } else {
       if (int rc = pk_grid(a, a.Tq, 128 / a.gp, a.units, name, &grid)) return rc;
       hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 4, BN>), dim3(grid), dim3(256), 0, stream, a);
@@ -1061,9 +1071,11 @@ template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, bool 
   }
   if (a.Tk > 0) {
     a.splits = parts;
-    if (few_keys) {
-      if (int rc = pk_grid(a, a.Tk, 32, nkh, name, &grid)) return rc;
-      hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 1, 1, false>), dim3(grid), dim3(64), 0, stream, a);
+    if (pk_few_keys<T, D>(a.Tk, a.S)) {
+      if constexpr (D <= 64 || sizeof(T) == 2) {
+        if (int rc = pk_grid(a, a.Tk, 32, nkh, name, &grid)) return rc;
+        hipLaunchKernelGGL((pk_bwd_dkv_kernel<T, D, 1, 1, false>), dim3(grid), dim3(64), 0, stream, a);
+      }
     } else {
       typedef DkvShape<T, D> SH;
       if (int rc = pk_grid(a, a.Tk, SH::KEYS, nkh, name, &grid)) return rc;
@@ -1100,5 +1112,5 @@ extern "C" int evlm_packed_attention_bwd(const evlm_packed_attn_args* x, void* s
     EVLM_REQUIRE(x->workspace, "%s: %d row parts need a workspace", name, parts);
     a.part = (float*)x->workspace;
   }
-  return PK_DISPATCH(x, pk_bwd_launch)(a, few, x->S > 0 && pk_few_keys(x), parts, (hipStream_t)stream_);
+  return PK_DISPATCH(x, pk_bwd_launch)(a, few, parts, (hipStream_t)stream_);
 }
