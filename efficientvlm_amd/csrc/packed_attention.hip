@@ -175,11 +175,52 @@ __device__ __forceinline__ Seq uniform(const Seq& x) {       // what every lane 
 __device__ __forceinline__ int vis_of(const PkArgs& a, const Seq& q, int tok) {
   return a.causal ? clampi(q.klen - q.qlen + tok + 1, 0, q.klen) : q.klen;
 }
+// ... one sequence after the other: every wave counts 64 E of them at a time, E a lane (24 tokens a sequence, 680 sequences, forward at
+// heads 16/4, dim 128: E = 4 92 us, E = 1 106 us; 65 sequences of 250: backward 114 and 107 us)
+template <bool KEYS, int E> __device__ __forceinline__ bool find_in_order(const PkArgs& a, int t, Seq& q, int& i, int& over, int& total) {
+  const int lane = threadIdx.x & 63;
+  int64_t before = 0;
+  for (int s0 = 0; s0 < a.S; s0 += 64 * E) {
+    int n[E];
+    int64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int s = s0 + E * lane + j;
+      n[j] = 0;
+      if (s < a.S) {
+        const Seq x = load_seq(a, s);
+        n[j] = ((KEYS ? x.klen : x.qlen) + a.per - 1) / a.per;
+      }
+      mine += n[j];
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    const unsigned long long hit = __ballot(before + incl > t);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      int64_t left = t - (before + incl - mine);             // (of the lane that has it: the block's index among the lane's)
+      int j = 0;
+#pragma unroll
+      for (int e = 0; e < E - 1; ++e)
+        if (j == e && left >= n[e]) { left -= n[e]; j = e + 1; }
+      q = uniform(load_seq(a, s0 + E * l + __shfl(j, l, 64)));
+      i = __builtin_amdgcn_readfirstlane(__shfl((int)left, l, 64));
+      return true;
+    }
+    before += __shfl(incl, 63, 64);
+  }
+  over = (int)(t - before);
+  total = (int)before;
+  return false;
+}
 // Block t of all sequences' blocks (KEYS: of their keys): the sequence it belongs to and its index there.  False: t lies behind the last
-// block (t - total in `over`), the block has nothing to do but the rows outside all sequences.  Every wave counts 64 sequences
-// at a time.  Up to 64 causal sequences are taken longest blocks first - the j-th block of queries, or the j-th block of keys from
-// the end, of every sequence that has one, j descending - so that the chip does not end on a few long blocks; of more
-// sequences, one after the other.
+// block (t - total in `over`), the block has nothing to do but the rows outside all sequences.  Up to 64 causal sequences are taken
+// longest blocks first - the j-th block of queries, or the j-th block of keys from the end, of every sequence that has one, j
+// descending - so that the chip does not end on a few long blocks; of more sequences, one after the other.
 template <bool KEYS> __device__ __forceinline__ bool find_tile(const PkArgs& a, int t, Seq& q, int& i, int& over, int& total) {
   const int lane = threadIdx.x & 63;
   if (a.causal && a.S <= 64) {
@@ -211,32 +252,7 @@ template <bool KEYS> __device__ __forceinline__ bool find_tile(const PkArgs& a, 
     i = __builtin_amdgcn_readfirstlane(KEYS ? __shfl(n, s, 64) - 1 - lo : lo);
     return true;
   }
-  int64_t before = 0;
-  for (int s0 = 0; s0 < a.S; s0 += 64) {
-    int n = 0;
-    if (s0 + lane < a.S) {
-      const Seq x = load_seq(a, s0 + lane);
-      n = ((KEYS ? x.klen : x.qlen) + a.per - 1) / a.per;
-    }
-    int64_t incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t up = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += up;
-    }
-    const unsigned long long hit = __ballot(before + incl > t);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int64_t first = before + __shfl(incl - n, l, 64);
-      q = uniform(load_seq(a, s0 + l));
-      i = __builtin_amdgcn_readfirstlane((int)(t - first));
-      return true;
-    }
-    before += __shfl(incl, 63, 64);
-  }
-  over = (int)(t - before);
-  total = (int)before;
-  return false;
+  return a.S > 128 ? find_in_order<KEYS, 4>(a, t, q, i, over, total) : find_in_order<KEYS, 1>(a, t, q, i, over, total);
 }
 // Few rows, many keys: the keys of every (sequence, block of tokens) are cut into chunks of one length for all, so that blocks of equal
 // work fill the chip however different the sequences are.  The length follows from the sequences themselves: their keys
