@@ -372,6 +372,30 @@ def test_join_with_the_hard_label_loss():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rest", [False, True])
+def test_a_gradient_larger_than_the_cache(dtype, rest):
+    """a thousand rows, and the same rows several times over with the loss's gradient as many times larger (powers of two: every
+    factor of a row is the same number): the same bits in each copy"""
+    C, k, n = 30001, 24, 8 if dtype == BF16 else 4
+    x = rows(1024, C, dtype, seed=9)
+    values, classes, lse = ops.top_logits(rows(1024, C, dtype, seed=10), k, temperature=2.0)
+    weight = torch.rand(1024, device="cuda")
+    weight[5] = 0.0
+
+    def grad(copies):
+        s = x.repeat(copies, 1).requires_grad_()
+        loss = ops.soft_cross_entropy_top(s, values.repeat(copies, 1), classes.repeat(copies, 1), lse=lse.repeat(copies) if rest else None,
+                                          temperature=2.0, row_weight=weight.repeat(copies))
+        return torch.autograd.grad(loss, s, torch.tensor(float(copies), device="cuda"))[0]
+
+    small, large = grad(1), grad(n)
+    assert (small.abs().sum(1) > 0).sum() == 1023
+    for i in range(n):
+        assert torch.equal(small, large[1024 * i:1024 * (i + 1)])
+
+
+@pytest.mark.gpu
 def test_same_bits_shapes_and_streams():
     s, v, c, l = pair(40, 3001, 32, BF16, seed=7)
     first = check_loss(s, v, c, l)
