@@ -481,10 +481,16 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
     st[ST_RAW_MAX] = m; st[ST_SWEEP_SUM] = sum; st[ST_P_REST] = (float)p_rest;
   }
 }
-__global__ __launch_bounds__(256) void kd_top_sum_kernel(const float* __restrict__ rowloss, int R, float coef, float* __restrict__ loss) {
+__global__ __launch_bounds__(1024) void kd_top_sum_kernel(const float* __restrict__ rowloss, int R, float coef, float* __restrict__ loss) {
   __shared__ float red[16];
   float s = 0.f;
-  for (int r = threadIdx.x; r < R; r += 256) s += rowloss[r];
+  for (int r = threadIdx.x; r < R; r += 8192) {              // (8 loads on their way at a time)
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = rowloss[min(r + 1024 * u, R - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += r + 1024 * u < R ? v[u] : 0.f;
+  }
   s = block_sum(s, red);
   if (threadIdx.x == 0) loss[0] = s * coef;
 }
@@ -591,7 +597,7 @@ extern "C" int evlm_kl_top_fwd(int dtype, const void* s, int R, int C, int64_t l
     else { if (lse_t) KDT_FWD(true, 0, bits); else KDT_FWD(false, 0, 0); })
 #undef KDT_FWD
   EVLM_LAUNCH_CHECK("evlm_kl_top_fwd");
-  hipLaunchKernelGGL(kd_top_sum_kernel, dim3(1), dim3(256), 0, stream, (const float*)rowloss, R, weight / (float)R, loss);
+  hipLaunchKernelGGL(kd_top_sum_kernel, dim3(1), dim3(1024), 0, stream, (const float*)rowloss, R, weight / (float)R, loss);
   EVLM_LAUNCH_CHECK("evlm_kl_top_fwd");
   return 0;
 }

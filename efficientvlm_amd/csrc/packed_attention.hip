@@ -168,6 +168,9 @@ __device__ __forceinline__ Seq load_seq(const PkArgs& a, int s) {
   if (a.k_lens) q.klen = clampi(a.k_lens[s], 0, q.klen);
   return q;
 }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
 __device__ __forceinline__ Seq uniform(const Seq& x) {       // what every lane holds alike, in scalar registers
   return Seq{__builtin_amdgcn_readfirstlane(x.qs), __builtin_amdgcn_readfirstlane(x.qlen), __builtin_amdgcn_readfirstlane(x.ks),
              __builtin_amdgcn_readfirstlane(x.klen)};
@@ -296,7 +299,7 @@ template <bool BY_TOKEN> __device__ __forceinline__ bool find_chunk(const PkArgs
       const int64_t rest = BY_TOKEN ? (int64_t)((g - c.q.qs) / a.per) * c.n : g - first;
       c.tile = __builtin_amdgcn_readfirstlane((int)(rest / c.n));
       c.chunk = __builtin_amdgcn_readfirstlane((int)(rest % c.n));
-      c.first = first + rest - rest % c.n;
+      c.first = uniform64(first + rest - rest % c.n);
       return true;
     }
     before += __shfl(incl, 63, 64);
@@ -461,7 +464,7 @@ template <typename T> __device__ __forceinline__ void fwd_outside(const PkArgs& 
 // forward, rows split over the waves: NW * 32 rows of one (sequence, chunk of heads), keys in shared blocks of BN
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BN>
-__global__ __launch_bounds__(64 * NW, 2) void pk_fwd_rows_kernel(PkArgs a) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) * D == 512 ? 1 : 2) void pk_fwd_rows_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
   __shared__ __attribute__((aligned(512))) char sm[2 * BN * TL::RB];
   char *Ks = sm, *Vs = sm + BN * TL::RB;
@@ -517,7 +520,7 @@ __device__ __forceinline__ float* part_of(const PkArgs& a, int64_t g, int unit) 
   return a.part + (g * a.units + unit) * (32 * (a.dh + 2));
 }
 template <typename T, int D, int NW, bool CH>
-__global__ __launch_bounds__(64 * NW, CH && sizeof(T) == 2 ? 2 : 1) void pk_fwd_keys_kernel(PkArgs a) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void pk_fwd_keys_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
   constexpr int WB = 2 * 32 * TL::RB > 32 * D * 4 ? 2 * 32 * TL::RB : 32 * D * 4;       // one wave's tiles, later its context
   __shared__ __attribute__((aligned(512))) char sm[NW * WB];
@@ -624,13 +627,28 @@ __global__ __launch_bounds__(64 * NW, CH && sizeof(T) == 2 ? 2 : 1) void pk_fwd_
   }
 }
 
-// join of the chunks: one wave per (token, head), lanes over the head dim.  Rows of one chunk are done; a token outside all sequences
-// is zero.  The parts' maxima and sums are read 64 chunks at a time, the parts themselves a few at once
+// v += f_i part_i for N parts, all on their way at a time (of the parts behind n the last is read again, their f is 0)
+template <int N> __device__ __forceinline__ void join_parts(const float* p, int64_t next, int n, unsigned d0, unsigned d1, float f, int i0, float& v0, float& v1) {
+  float x0[N], x1[N];
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const float* pi = p + min(u, n - 1) * next;
+    x0[u] = pi[d0]; x1[u] = pi[d1];
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (i0 + u) & 63));      // (0 in the lanes behind the last part)
+    v0 = fmaf(x0[u], fi, v0);
+    v1 = fmaf(x1[u], fi, v1);
+  }
+}
+// join of the chunks: one wave per (token, head), lanes over the head dim, 4 heads a block.  Rows of one chunk are done; a token
+// outside all sequences is zero.  The parts' maxima and sums are read 64 chunks at a time, the parts themselves eight or four at once
 template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.Tq * a.H) return;
+  const unsigned per = (a.H + 3) / 4;
+  const int t = blockIdx.x / per, h = __builtin_amdgcn_readfirstlane((int)(blockIdx.x % per * 4 + (threadIdx.x >> 6)));
+  if (h >= a.H) return;
   const int lane = threadIdx.x & 63;
-  const int t = __builtin_amdgcn_readfirstlane((int)(row / a.H)), h = __builtin_amdgcn_readfirstlane((int)(row % a.H));
   Chunk c;
   const bool inside = find_chunk<true>(a, t, c);
   if (inside && c.n == 1) return;
@@ -638,10 +656,12 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
   float M = -INFINITY, L = 0.f, v0 = 0.f, v1 = 0.f;
   if (inside) {
     const int unit = h / a.gp, r = (t - c.q.qs - c.tile * a.per) * a.gp + h % a.gp;      // (heads of a unit are consecutive)
-    const int n = (int)min((int64_t)c.n, a.tiles - c.first);                             // (never past the workspace)
+    const int n = __builtin_amdgcn_readfirstlane((int)min((int64_t)c.n, a.tiles - c.first));                             // (never past the workspace)
     for (int i = lane; i < n; i += 64) M = fmaxf(M, part_of(a, c.first + i, unit)[32 * a.dh + 2 * r]);
     M = wave_max(M);
     if (M != -INFINITY) {
+      const unsigned d0 = min(lane, a.dh - 1), d1 = min(lane + 64, a.dh - 1);
+      const int64_t next = (int64_t)a.units * (32 * (a.dh + 2));
       for (int i0 = 0; i0 < n; i0 += 64) {
         float f = 0.f;
         if (i0 + lane < n) {
@@ -650,14 +670,10 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
           L = fmaf(ml[1], f, L);
         }
         const int e = min(64, n - i0);
-        const float* p = part_of(a, c.first + i0, unit) + r * a.dh;
-        const int64_t next = (int64_t)a.units * (32 * (a.dh + 2));
-        const int d0 = min(lane, a.dh - 1), d1 = min(lane + 64, a.dh - 1);
-        for (int i = 0; i < e; ++i) {
-          const float fi = __shfl(f, i, 64);
-          v0 = fmaf(p[i * next + d0], fi, v0);
-          v1 = fmaf(p[i * next + d1], fi, v1);
-        }
+        const float* p = (const float*)uniform64((int64_t)(part_of(a, c.first + i0, unit) + r * a.dh));
+        int i = 0;
+        for (; i + 8 <= e; i += 8) join_parts<8>(p + i * next, next, 8, d0, d1, f, i, v0, v1);
+        for (; i < e; i += 4) join_parts<4>(p + i * next, next, e - i, d0, d1, f, i, v0, v1);
       }
       L = wave_sum(L);
     }
@@ -675,14 +691,18 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward, dQ: NW * 32 rows as in the forward; delta = dO.O of the block's rows is formed here and kept for dK / dV
+// backward, dQ: NW * 32 rows as in the forward (KS: 32 rows, every wave with keys of its own, the waves' sums joined at the end);
+// delta = dO.O of the block's rows is formed here and kept for dK / dV.  Two waves a SIMD; the joined one at head dim 128 is faster
+// with one and no spills (32 sequences of 8 queries and 500 keys, heads 16/4, both directions: 73 and 83 us)
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int NW, int BN>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_kernel(PkArgs a) {
+template <typename T, int D, int NW, int BN, bool KS>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 128) ? 1 : 2) void pk_bwd_dq_kernel(PkArgs a) {
   typedef Tile<T, D> TL;
-  __shared__ __attribute__((aligned(512))) char sm[2 * BN * TL::RB];
-  char *Ks = sm, *Vs = sm + BN * TL::RB;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  constexpr int WB = 2 * BN * TL::RB, NT = KS ? 64 : 64 * NW;                   // KS: a wave has keys of its own, staged by itself
+  __shared__ __attribute__((aligned(512))) char sm[(KS ? NW : 1) * WB];
+  const int own = KS ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  char *Ks = sm + own * WB, *Vs = Ks + BN * TL::RB;
+  const int tid = threadIdx.x & (NT - 1), lane = tid & 63, wave = KS ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const int unit = blockIdx.x % a.units, kh = unit / a.chunks, h0 = kh * a.G + (unit % a.chunks) * a.gp;
   Seq q; int ti, over, total;
   if (!find_tile<false>(a, blockIdx.x / a.units, q, ti, over, total)) {
@@ -719,20 +739,22 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
         for (int j = 0; j < TL::EP; ++j) delta = fmaf((float)df[s][j], (float)of[s][j], delta);
     }
     delta += __shfl_xor(delta, 32, 64);
-    if (valid && hh == 0) a.delta[(int64_t)h * a.Tq + t] = delta;
+    if (valid && hh == 0 && own == 0) a.delta[(int64_t)h * a.Tq + t] = delta;
   }
   const float lse = valid ? a.lse[(int64_t)h * a.Tq + t] : INFINITY;
   const T* Kb = (const T*)a.K + q.ks * a.k_tok + kh * a.k_head;
   const T* Vb = (const T*)a.V + q.ks * a.v_tok + kh * a.v_head;
   f32x16 acc[D / 32] = {};
-  Stage<T, D, BN, 64 * NW> ks, vs;
-  if (nk > 0) { ks.load(Kb, a.k_tok, 0, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, 0, q.klen, a.dh, tid); }
-  for (int kt = 0; kt < nk; kt += BN) {
-    __syncthreads();
+  Stage<T, D, BN, NT> ks, vs;
+  constexpr int STEP = KS ? NW * BN : BN;
+  int kt = own * BN;
+  if (kt < nk) { ks.load(Kb, a.k_tok, kt, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, kt, q.klen, a.dh, tid); }
+  for (; kt < nk; kt += STEP) {
+    if constexpr (KS) wave_lds_fence(); else __syncthreads();
     ks.pad(a.dh, tid); vs.pad(a.dh, tid);
     ks.store(Ks, tid); vs.store(Vs, tid);
-    __syncthreads();
-    if (kt + BN < nk) { ks.load(Kb, a.k_tok, kt + BN, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, kt + BN, q.klen, a.dh, tid); }
+    if constexpr (KS) wave_lds_fence(); else __syncthreads();
+    if (kt + STEP < nk) { ks.load(Kb, a.k_tok, kt + STEP, q.klen, a.dh, tid); vs.load(Vb, a.v_tok, kt + STEP, q.klen, a.dh, tid); }
     if (w_any && kt < w_max) {
       const bool mask = kt + BN > w_min;
 #pragma unroll
@@ -749,7 +771,29 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void pk_bwd_dq_ker
       }
     }
   }
-  if (valid) store_cols<T, D>((T*)a.dQ + t * a.dq_tok + h * a.dq_head, a.dh, acc, a.scale, hh);
+  T* out = (T*)a.dQ + t * a.dq_tok + h * a.dq_head;
+  if constexpr (KS && NW > 1) {                              // join the waves, thread -> (row, 4 consecutive d)
+    wave_lds_fence();
+    float* mine = (float*)(sm + own * WB);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine[(dt * 32 + c_row(i, hh)) * 32 + r] = acc[dt][i];
+    __syncthreads();
+    if (!valid) return;
+    for (int d = (own * 2 + hh) * 4; d < a.dh; d += NW * 8) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += ((float*)(sm + w * WB))[(d + j) * 32 + r];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] *= a.scale;
+      Vec4<T>::store(out + d, v);
+    }
+  } else {
+    if (valid) store_cols<T, D>(out, a.dh, acc, a.scale, hh);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -936,12 +980,16 @@ static bool pk_few_rows(const evlm_packed_attn_args* x, int gp) {
   // rows of a sequence and chunk of heads, on average: one wave's worth -> keys are split over the waves instead of rows
   return (int64_t)x->Tq * gp <= (int64_t)48 * x->S;
 }
-// chunks of keys aimed at for each chunk of heads; 0: every block of rows walks all its keys.  Worth it where a sequence has room for
-// more than two chunks and the rows alone are few blocks
+// chunks of keys aimed at for each chunk of heads; 0: every block of rows walks all its keys.  Worth it where the rows alone are too few
+// blocks for the chip, or are of very different lengths and long enough to pay for the second kernel.  Single tokens, heads 32/8 of 128,
+// lengths between a third and five thirds of the mean, us with / without chunks: 800 keys, 72 blocks 34 / 33, 288: 37 / 28; 2000 keys,
+// 144: 43 / 38, 576: 122 / 124; 8000 keys, 144: 126 / 185, 576: 438 / 487, 1152: 903 / 928.  12 sequences of 6 000 - 40 000 keys (104
+// blocks): 137 / 400.  30 rows on 577 keys, heads 12/12 of 64, 1488: 61 / 34
 static int pk_want(const evlm_packed_attn_args* x, int gp) {
   if (x->S == 0 || x->Tq == 0 || !pk_few_rows(x, gp) || (int64_t)x->Tk <= (int64_t)2 * PK_CHUNK * x->S) return 0;
-  const int64_t units = x->H / gp, rows = ((int64_t)x->Tq * gp / 32 + x->S) * units;
-  return rows >= 2048 ? 0 : (int)((PK_BLOCKS + units - 1) / units);
+  const int64_t units = x->H / gp, blocks = ((int64_t)x->Tq * gp / 32 + x->S) * units;
+  const bool wanted = blocks < 128 || (blocks < 1024 && (int64_t)x->Tk >= (int64_t)4096 * x->S);
+  return wanted ? (int)((PK_BLOCKS + units - 1) / units) : 0;
 }
 static int64_t pk_chunk_slots(const evlm_packed_attn_args* x, int gp) {     // an upper bound of the chunks, whatever the lengths
   return pk_want(x, gp) + (int64_t)x->Tq / (32 / gp) + x->S;
@@ -1029,8 +1077,8 @@ template <typename T, int D> static int pk_fwd_launch(PkArgs& a, bool few, int64
     a.tiles = (int)slots;
     hipLaunchKernelGGL((pk_fwd_keys_kernel<T, D, 4, true>), dim3((unsigned)(slots * a.units)), dim3(256), 0, stream, a);
     EVLM_LAUNCH_CHECK("evlm_packed_attention_fwd");
-    const int64_t rows = (int64_t)a.Tq * a.H;
-    hipLaunchKernelGGL((pk_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+    const int64_t blocks = (int64_t)a.Tq * ((a.H + 3) / 4);
+    hipLaunchKernelGGL((pk_join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
   } else if (few) {
     if (int rc = pk_grid(a, a.Tq, 32 / a.gp, a.units, "evlm_packed_attention_fwd", &grid)) return rc;
     if (a.S > 0 && a.Tk / a.S <= 64)
@@ -1071,17 +1119,21 @@ template <typename T, int D> static int pk_bwd_launch(PkArgs& a, bool few, int p
   const char* name = "evlm_packed_attention_bwd";
   const int nkh = a.H / a.G;
   if (a.Tq > 0) {
-    // one wave a block for few rows (16 384 tokens, heads 8/8, 24 a sequence, bf16 dim 128: backward 171 us, 224 with blocks of four),
-    // but not at dim 128 in f32, where it spilled (4096 tokens, heads 16/4, 24 a sequence: 267 us, 227 with blocks of four)
+    // few rows: one wave a block (16 384 tokens, heads 8/8, 24 a sequence, bf16 dim 128: backward 171 us, 224 with 128-row blocks), but
+    // not at dim 128 in f32, where it spilled (4096 tokens, heads 16/4, 24 a sequence: 267 us, 227 with 128-row blocks).  Its keys
+    // split over four waves where they are many and the blocks would not give every SIMD a wave (both directions, 9 sequences of 47
+    // queries and 210 keys, 12 heads of 64 in f32: 60 us, 83 with one wave; 64 sequences of 30 and 577 in bf16, 768 blocks: 270, 264)
     constexpr bool kOneWave = D <= 64 || sizeof(T) == 2;
+    const bool split = few && a.Tk / a.S > 64 && ((int64_t)a.Tq * a.gp / 32 + a.S) * a.units <= 1024;
     if (few && kOneWave) {
       if constexpr (kOneWave) {
         if (int rc = pk_grid(a, a.Tq, 32 / a.gp, a.units, name, &grid)) return rc;
-        hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 1, 32>), dim3(grid), dim3(64), 0, stream, a);
+        if (split) hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 4, 32, true>), dim3(grid), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 1, 32, true>), dim3(grid), dim3(64), 0, stream, a);
       }
     } else {
       if (int rc = pk_grid(a, a.Tq, 128 / a.gp, a.units, name, &grid)) return rc;
-      hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 4, BN>), dim3(grid), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((pk_bwd_dq_kernel<T, D, 4, BN, false>), dim3(grid), dim3(256), 0, stream, a);
     }
     EVLM_LAUNCH_CHECK(name);
   }
