@@ -231,6 +231,33 @@ def test_few_tokens_behind_caches_train(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,dh,lq,lk", [
+    ((2, 1), 128, [255, 256, 257, 31, 1], None),                         # blocks of 256 keys and of 128
+    ((4, 1), 128, [600, 90], None),                                      # ... their rows shared by several blocks
+    ((4, 1), 128, [20, 47, 1, 33], None),                                # ... and of 32
+    ((2, 2), 64, [150, 161, 32, 33], None),                              # one wave a block of keys, several blocks
+    ((2, 2), 64, [300, 210, 128], None),                                 # four waves a block of keys
+    ((4, 2), 64, [3, 1, 0, 30, 17], [65, 700, 100, 333, 0]),             # few queries: keys split over the waves
+    ((4, 2), 128, [3, 1, 0, 30, 17], [65, 700, 100, 333, 0]),
+    ((8, 8), 32, [7] * 135, [70] * 134 + [40]),                          # ... enough blocks without; sequences counted four a lane
+    ((2, 1), 64, [9, 40, 1] * 30, None),                                 # 90 sequences, in order
+])
+def test_forms_of_the_work(dtype, causal, heads, dh, lq, lk):
+    """lengths around the sizes at which the kernels cut the work differently"""
+    both(problem(dtype, *heads, dh, lq, lk, seed=len(lq)), causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("parts", [1, 3, 4, 7, 8, 9, 30, 75])
+def test_chunks_of_keys_joined(dtype, parts):
+    """a single token over so many chunks (one chunk a head group is at least 256 keys)"""
+    both(problem(dtype, 2, 1, 72, [1, 2], [256 * parts, 600], slots=3), backward=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("layout", ["qkv", "heads_first", "odd"])
 def test_layouts(dtype, layout):
     p = problem(dtype, 4, 2, 64, [40, 9, 150], layout=layout)
