@@ -247,6 +247,12 @@ def test_loss_sizes(dtype, rest, R, C, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R", [1023, 8192, 9001])
+def test_loss_of_many_rows(R):
+    check_loss(*pair(R, 9, 4, F32, seed=R, rest=True))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_all_classes_kept_is_the_whole_rows_loss(dtype):
     """k = C: soft_cross_entropy of the same logits"""
