@@ -92,7 +92,8 @@ __device__ __forceinline__ int block_count(int v, int* red) {
 // Rows with long ties at the bound (more candidates than the list holds) and rows with NaN or without a finite maximum get the
 // exact bound by bisection over the row, first of the value, then of the class among equals.
 // Bound by its vector instructions as much as by HBM: 8 elements cost 12 instructions for the maximum, 56 slots for the sum and
-// one compare against the bound (their maximum is kept).
+// one compare against the bound (their maximum is kept).  3000 bf16 rows of 30 522, k = 64: 56 us = 3.3 TB/s; 7 rows: 8.9 us, the
+// phases of one row after the other.
 #define TOP_NT 512
 #define TOP_CAP 1024
 #define TOP_LOG2E 1.44269504088896341f
@@ -302,7 +303,8 @@ __device__ __forceinline__ double wave_max_f64(double v) {
 }
 __device__ __forceinline__ float exp_from(float x, float m) { return x == -INFINITY ? 0.f : __expf(x - m); }   // exp(x - m), x <= m
 
-// NCH > 0: rows of up to NCH * 8 * KDT_NT elements are asked for before anything else and stay in registers
+// NCH > 0: rows of up to NCH * 8 * KDT_NT elements are asked for before anything else and stay in registers.
+// One read of the logits; 5000 bf16 rows of 30 522 with 64 kept: 77 us = 4.0 TB/s (the exponentials as in the selection), 330 rows 13 us
 template <typename T, bool REST, int NCH>
 __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void kd_top_fwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, const float* __restrict__ lse_t,
@@ -511,6 +513,7 @@ template <typename T> __device__ __forceinline__ void store8_past(T* p, const fl
 // Rows are taken from the last to the first: the forward sweep left the last ones in the 256 MB cache.  NT: a gradient that does not
 // fit into that cache is stored past it, and the logits stay (bf16, 30 522 classes, 5000 rows, both directions: 198 us; with
 // plain stores 207, first row first as well 213; 12 000 rows 453, 484, 488).  A smaller one is read from there by the next product.
+// Bound by HBM: 107 us alone for 610 MB (5.7 TB/s).
 template <typename T, bool REST, bool NT>
 __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, int k, float inv_t, float coef,
