@@ -16,6 +16,8 @@
 #include "common.h"
 
 #define TOP_MAX_K 256
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 // 8 consecutive elements of a row from any element-aligned address
 template <typename T> __device__ __forceinline__ void load8_any(const T* p, float v[8]);
@@ -97,21 +99,36 @@ __device__ __forceinline__ int block_count(int v, int* red) {
 #define TOP_NT 512
 #define TOP_CAP 1024
 #define TOP_LOG2E 1.44269504088896341f
+// maximum of two as the median with +inf: one instruction, where fmaxf first quiets what may be a signalling NaN.  (One NaN: the
+// other; two: +inf.  The sum of such a row is NaN, and nothing is done with its maximum.)
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 __device__ __forceinline__ float max8(const float (&v)[8]) {
-  return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+  return max_of(max_of(max_of(v[0], v[1]), max_of(v[2], v[3])), max_of(max_of(v[4], v[5]), max_of(v[6], v[7])));
 }
-// exp((v - m) / T), c2 = log2e / T.  (The difference first: a maximum of the type's lowest value times log2e would be -inf.)
+// exp((v - m) / T) = 2^((v - m) c2), c2 = log2e / T
 __device__ __forceinline__ float exp_diff(float v, float m, float c2) { return __builtin_amdgcn_exp2f((v - m) * c2); }
+// Sums of it over a row: v c2 - m c2 in one fma, and the sum afterwards by what the rounding of m c2 left (tail), so that it is as exact as
+// with the difference first.  Where m c2 is out of range (a maximum of the type's lowest value), the difference first.
+struct ExpSum {
+  float m, c2, off;
+  bool in_range;
+  __device__ __forceinline__ ExpSum(float m_, float c2_) : m(m_), c2(c2_), off(-m_ * c2_), in_range(fabsf(m_ * c2_) < 1e30f) {}
+  __device__ __forceinline__ float tail() const { return in_range ? __builtin_amdgcn_exp2f(-fmaf(m, c2, off)) : 1.0f; }
+  template <bool FAST> __device__ __forceinline__ float of(float v) const {
+    return FAST ? __builtin_amdgcn_exp2f(fmaf(v, c2, off)) : exp_diff(v, m, c2);
+  }
+};
 template <typename T, int NCH>
-__global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict__ logits, int C, int64_t ld, int k, float inv_t,
+__global__ __launch_bounds__(TOP_NT, sizeof(T) == 2 ? 8 : 4) void top_logits_kernel(const T* __restrict__ logits, int C, int64_t ld, int k, float inv_t,
                                                             float* __restrict__ values, int32_t* __restrict__ classes,
                                                             float* __restrict__ lse) {
   __shared__ float red[16];
   __shared__ int ired[16];
   __shared__ uint32_t tops[TOP_NT];
   __shared__ unsigned long long list[TOP_CAP];
+  __shared__ uint32_t hits[TOP_CAP];
   __shared__ uint32_t bound;
-  __shared__ int count;
+  __shared__ int count, nhits;
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t r = blockIdx.x;
   const T* x = logits + r * ld;
@@ -140,14 +157,14 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
         float v[8];
         keep[n].get(v);
         most[n] = max8(v);
-        mx = fmaxf(mx, most[n]);
+        mx = max_of(mx, most[n]);
       }
     }
   } else {
-    again([&](const float (&v)[8], int) { mx = fmaxf(mx, max8(v)); });
+    again([&](const float (&v)[8], int) { mx = max_of(mx, max8(v)); });
   }
   tops[tid] = tid < chunks ? order_key(mx) : 0u;
-  if (tid == 0) count = 0;
+  if (tid == 0) { count = 0; nhits = 0; }
   const float M = block_max(mx, red);                        // (ends the hand-over of tops and count, too)
   if (tid < 64) {
     uint32_t t[TOP_NT / 64], b = 0;
@@ -163,47 +180,57 @@ __global__ __launch_bounds__(TOP_NT) void top_logits_kernel(const T* __restrict_
     if (lane == 0) bound = b;
   }
   // sum of exp((v - M) / T): NaN where the row holds one, or has no finite maximum
-  const float c2 = inv_t * TOP_LOG2E;
+  const ExpSum ex(M, inv_t * TOP_LOG2E);
   float s = 0.f;
-  auto add8 = [&](const float (&v)[8], int) __attribute__((always_inline)) {
+  auto sweep = [&](auto fast) __attribute__((always_inline)) {
+    auto add8 = [&](const float (&v)[8], int) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += exp_diff(v[e], M, c2);
-  };
-  if constexpr (NCH > 0) {
-#pragma unroll
-    for (int n = 0; n < NCH; ++n)
-      if (tid + n * TOP_NT < chunks) {
-        float v[8];
-        keep[n].get(v);
-        add8(v, 0);
-      }
-  } else {
-    again(add8);
-  }
-  s = block_sum(s, red);
-  const bool regular = s < INFINITY;                         // (block-uniform; false for NaN)
-  if (regular) {
-    if (tid == 0) lse[r] = M * inv_t + logf(s);
-    const float b = key_value(max(bound, 0x00800000u));      // (the lowest finite value at least)
-    auto collect = [&](const float (&v)[8], int i0) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v[e] >= b && i0 + e < C) {
-          const int at = atomicAdd(&count, 1);
-          if (at < TOP_CAP) list[at] = ((unsigned long long)order_key(v[e]) << 32) | (uint32_t)~(i0 + e);
-        }
+      for (int e = 0; e < 8; ++e) s += ex.template of<decltype(fast)::value>(v[e]);
     };
     if constexpr (NCH > 0) {
 #pragma unroll
       for (int n = 0; n < NCH; ++n)
-        if (most[n] >= b) {
+        if (tid + n * TOP_NT < chunks) {
           float v[8];
           keep[n].get(v);
-          collect(v, 8 * (tid + n * TOP_NT));
+          add8(v, 0);
         }
     } else {
-      again([&](const float (&v)[8], int i0) { if (max8(v) >= b) collect(v, i0); });
+      again(add8);
     }
+  };
+  if (ex.in_range) sweep(Yes()); else sweep(No());           // (block-uniform)
+  s = block_sum(s, red) * ex.tail();
+  const bool regular = s < INFINITY;                         // (block-uniform; false for NaN)
+  if (regular) {
+    if (tid == 0) lse[r] = M * inv_t + logf(s);
+    const float b = key_value(max(bound, 0x00800000u));      // (the lowest finite value at least)
+    // the pieces of 8 that hold a candidate, then their elements, one a thread (asked for again: few)
+    auto hit = [&](int c) __attribute__((always_inline)) {
+      const int at = atomicAdd(&nhits, 1);
+      if (at < TOP_CAP) hits[at] = c;
+    };
+    if constexpr (NCH > 0) {
+#pragma unroll
+      for (int n = 0; n < NCH; ++n)
+        if (most[n] >= b) hit(tid + n * TOP_NT);
+    } else {
+      again([&](const float (&v)[8], int i0) { if (max8(v) >= b) hit(i0 >> 3); });
+    }
+    __syncthreads();
+    const int pieces = nhits;
+    if (pieces > TOP_CAP) { if (tid == 0) count = TOP_CAP + 1; }
+    else
+      for (int i = tid; i < 8 * pieces; i += TOP_NT) {
+        const int e = 8 * (int)hits[i >> 3] + (i & 7);
+        if (e < C) {
+          const float v = to_f(x[e]);
+          if (v >= b) {
+            const int at = atomicAdd(&count, 1);
+            if (at < TOP_CAP) list[at] = ((unsigned long long)order_key(v) << 32) | (uint32_t)~e;
+          }
+        }
+      }
   } else {
     int nan = 0;
     again([&](const float (&v)[8], int) {
@@ -355,7 +382,6 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
     __syncthreads();
   }
   // maximum and sum of the row (REST: of the classes that are not kept), thread by thread
-  const float c2 = inv_t * TOP_LOG2E;
   auto drop_kept = [&](float (&v)[8], int c) __attribute__((always_inline)) {
     if constexpr (REST) {
       const uint32_t bits = (kept[c >> 2] >> (8 * (c & 3))) & 0xFFu;
@@ -380,7 +406,7 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
             for (int e = 0; e < 8; ++e) keep[n].set(e, from_f<T>(v[e]));
           }
         }
-        m = fmaxf(m, max8(v));
+        m = max_of(m, max8(v));
       }
     }
   } else {
@@ -388,29 +414,32 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
       float v[8];
       row8<T>(x, c, C, -INFINITY, v);
       drop_kept(v, c);
-      m = fmaxf(m, max8(v));
+      m = max_of(m, max8(v));
     }
   }
   m = block_max(m, red);
-  const float base = m == -INFINITY ? 0.f : m;
-  if constexpr (NCH > 0) {
+  const ExpSum ex(m == -INFINITY ? 0.f : m, inv_t * TOP_LOG2E);
+  auto sweep = [&](auto fast) __attribute__((always_inline)) {
+    if constexpr (NCH > 0) {
 #pragma unroll
-    for (int n = 0; n < NCH; ++n)
-      if (tid + n * KDT_NT < chunks) {
+      for (int n = 0; n < NCH; ++n)
+        if (tid + n * KDT_NT < chunks) {
+          float v[8];
+          keep[n].get(v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += ex.template of<decltype(fast)::value>(v[e]);
+        }
+    } else {
+      for (int c = tid; c < chunks; c += KDT_NT) {
         float v[8];
-        keep[n].get(v);
+        row8<T>(x, c, C, -INFINITY, v);
+        drop_kept(v, c);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += exp_diff(v[e], base, c2);
+        for (int e = 0; e < 8; ++e) sum += ex.template of<decltype(fast)::value>(v[e]);
       }
-  } else {
-    for (int c = tid; c < chunks; c += KDT_NT) {
-      float v[8];
-      row8<T>(x, c, C, -INFINITY, v);
-      drop_kept(v, c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += exp_diff(v[e], base, c2);
     }
-  }
+  };
+  if (ex.in_range) sweep(Yes()); else sweep(No());           // (block-uniform)
   float z[NE], y[NE];
   if (tid < 64) {
 #pragma unroll
@@ -419,7 +448,7 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
       y[i] = ci[i] >= 0 ? to_f(x[ci[i]]) : 0.f;
     }
   }
-  sum = block_sum(sum, red);                                 // (NaN where the row holds one)
+  sum = block_sum(sum, red) * ex.tail();                     // (NaN where the row holds one)
   if (tid >= 64) return;                                     // the rest is the first wave's
   // A student close to its teacher has a loss of a few per thousand, the difference of terms of size 1, and p_rest is what is left
   // of 1: the k + 1 terms are formed in 64 bits (32 kept four digits of such a row's loss).
