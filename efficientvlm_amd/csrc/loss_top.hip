@@ -49,6 +49,17 @@ template <> struct TopRaw8<bf16> {
     for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
   }
   __device__ __forceinline__ void set(int i, bf16 x) { t[i] = x; }
+  __device__ __forceinline__ void drop(uint32_t bits) {      // -inf where the bit is set (a select by masks: 4 instructions a pair)
+    uint32_t w[4];
+    __builtin_memcpy(w, &t, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = __builtin_amdgcn_sbfe((int)bits, 2 * i, 1), hi = __builtin_amdgcn_sbfe((int)bits, 2 * i + 1, 1);
+      const uint32_t mask = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
+      w[i] = (mask & 0xFF80FF80u) | (~mask & w[i]);
+    }
+    __builtin_memcpy(&t, w, 16);
+  }
 };
 template <> struct TopRaw8<float> {
   f32x4 t[2];
@@ -57,6 +68,10 @@ template <> struct TopRaw8<float> {
     for (int i = 0; i < 8; ++i) v[i] = t[i >> 2][i & 3];
   }
   __device__ __forceinline__ void set(int i, float x) { t[i >> 2][i & 3] = x; }
+  __device__ __forceinline__ void drop(uint32_t bits) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i >> 2][i & 3] = (bits >> i) & 1u ? -INFINITY : t[i >> 2][i & 3];
+  }
 };
 template <typename T> __device__ __forceinline__ void raw8(const T* x, int c, int C, float fill, TopRaw8<T>& o) {
   if (8 * c + 8 <= C) { __builtin_memcpy(&o, x + 8 * (int64_t)c, sizeof(o)); return; }
@@ -93,17 +108,39 @@ __device__ __forceinline__ int block_count(int v, int* red) {
 // counting, (value, lower class first) making every element distinct - the result does not depend on the order of collection.
 // Rows with long ties at the bound (more candidates than the list holds) and rows with NaN or without a finite maximum get the
 // exact bound by bisection over the row, first of the value, then of the class among equals.
-// Bound by its vector instructions as much as by HBM: 8 elements cost 12 instructions for the maximum, 56 slots for the sum and
-// one compare against the bound (their maximum is kept).  3000 bf16 rows of 30 522, k = 64: 56 us = 3.3 TB/s; 7 rows: 8.9 us, the
-// phases of one row after the other.
+// Bound by its vector instructions beside HBM: 8 elements cost 14 instructions for the maximum (which is kept) and 56 slots for the sum (an
+// exponential takes four); the candidates are collected by pieces of 8 first (one compare a piece), then one element a thread: with every
+// thread testing the 8 of its own pieces, a wave went through nearly all of them for two or three candidates.
+// 3000 bf16 rows of 30 522, k = 64: 47 us = 3.9 TB/s (56 before these three); 7 rows: 8.9 us, the phases of one row after the other.
 #define TOP_NT 512
 #define TOP_CAP 1024
 #define TOP_LOG2E 1.44269504088896341f
-// maximum of two as the median with +inf: one instruction, where fmaxf first quiets what may be a signalling NaN.  (One NaN: the
-// other; two: +inf.  The sum of such a row is NaN, and nothing is done with its maximum.)
-__device__ __forceinline__ float max_of(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 __device__ __forceinline__ float max8(const float (&v)[8]) {
-  return max_of(max_of(max_of(v[0], v[1]), max_of(v[2], v[3])), max_of(max_of(v[4], v[5]), max_of(v[6], v[7])));
+  return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+}
+__device__ __forceinline__ float max8(const TopRaw8<float>& x) {
+  float v[8];
+  x.get(v);
+  return max8(v);
+}
+// bf16: their patterns two at a time.  As signed numbers the patterns of positive values are in order and above those of negative ones; among
+// negative ones the smallest unsigned pattern is the largest value.  (14 instructions for the 8, where as floats - each is
+// quieted first - they took 32.  A NaN may win or not: the sum of its row is NaN, and nothing is done with the maximum.)
+__device__ __forceinline__ float max8(const TopRaw8<bf16>& x) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  uint32_t w[4];
+  __builtin_memcpy(w, &x.t, 16);
+  s16x2 hi = __builtin_bit_cast(s16x2, w[0]);
+  u16x2 lo = __builtin_bit_cast(u16x2, w[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    hi = __builtin_elementwise_max(hi, __builtin_bit_cast(s16x2, w[i]));
+    lo = __builtin_elementwise_min(lo, __builtin_bit_cast(u16x2, w[i]));
+  }
+  const int h = hi[0] > hi[1] ? hi[0] : hi[1];
+  const unsigned l = lo[0] < lo[1] ? lo[0] : lo[1];
+  return __uint_as_float((h >= 0 ? (unsigned)h : l) << 16);
 }
 // exp((v - m) / T) = 2^((v - m) c2), c2 = log2e / T
 __device__ __forceinline__ float exp_diff(float v, float m, float c2) { return __builtin_amdgcn_exp2f((v - m) * c2); }
@@ -154,14 +191,12 @@ __global__ __launch_bounds__(TOP_NT, sizeof(T) == 2 ? 8 : 4) void top_logits_ker
     for (int n = 0; n < NCH; ++n) {
       most[n] = -INFINITY;
       if (tid + n * TOP_NT < chunks) {
-        float v[8];
-        keep[n].get(v);
-        most[n] = max8(v);
-        mx = max_of(mx, most[n]);
+        most[n] = max8(keep[n]);
+        mx = fmaxf(mx, most[n]);
       }
     }
   } else {
-    again([&](const float (&v)[8], int) { mx = max_of(mx, max8(v)); });
+    again([&](const float (&v)[8], int) { mx = fmaxf(mx, max8(v)); });
   }
   tops[tid] = tid < chunks ? order_key(mx) : 0u;
   if (tid == 0) { count = 0; nhits = 0; }
@@ -331,7 +366,8 @@ __device__ __forceinline__ double wave_max_f64(double v) {
 __device__ __forceinline__ float exp_from(float x, float m) { return x == -INFINITY ? 0.f : __expf(x - m); }   // exp(x - m), x <= m
 
 // NCH > 0: rows of up to NCH * 8 * KDT_NT elements are asked for before anything else and stay in registers.
-// One read of the logits; 5000 bf16 rows of 30 522 with 64 kept: 77 us = 4.0 TB/s (the exponentials as in the selection), 330 rows 13 us
+// One read of the logits, bound by HBM and, nearly, by its vector instructions (as the selection): 5000 bf16 rows of 30 522 with 64 kept
+// 70 us = 4.4 TB/s, 12 000 155 us = 4.7 TB/s; 330 rows 12 us.
 template <typename T, bool REST, int NCH>
 __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void kd_top_fwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, const float* __restrict__ lse_t,
@@ -397,16 +433,11 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
     for (int n = 0; n < NCH; ++n) {
       const int c = tid + n * KDT_NT;
       if (c < chunks) {
-        float v[8];
-        keep[n].get(v);
         if constexpr (REST) {
-          if ((kept[c >> 2] >> (8 * (c & 3))) & 0xFFu) {
-            drop_kept(v, c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) keep[n].set(e, from_f<T>(v[e]));
-          }
+          const uint32_t bits = (kept[c >> 2] >> (8 * (c & 3))) & 0xFFu;
+          if (bits) keep[n].drop(bits);
         }
-        m = max_of(m, max8(v));
+        m = fmaxf(m, max8(keep[n]));
       }
     }
   } else {
@@ -414,7 +445,7 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
       float v[8];
       row8<T>(x, c, C, -INFINITY, v);
       drop_kept(v, c);
-      m = max_of(m, max8(v));
+      m = fmaxf(m, max8(v));
     }
   }
   m = block_max(m, red);
