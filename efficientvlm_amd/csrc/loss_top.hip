@@ -111,7 +111,7 @@ __device__ __forceinline__ int block_count(int v, int* red) {
 // Bound by its vector instructions beside HBM: 8 elements cost 14 instructions for the maximum (which is kept) and 56 slots for the sum (an
 // exponential takes four); the candidates are collected by pieces of 8 first (one compare a piece), then one element a thread: with every
 // thread testing the 8 of its own pieces, a wave went through nearly all of them for two or three candidates.
-// 3000 bf16 rows of 30 522, k = 64: 47 us = 3.9 TB/s (56 before these three); 7 rows: 8.9 us, the phases of one row after the other.
+// 3000 bf16 rows of 30 522, k = 64: 44 us = 4.2 TB/s (56 before these three); 7 rows: 7.8 us, the phases of one row after the other.
 #define TOP_NT 512
 #define TOP_CAP 1024
 #define TOP_LOG2E 1.44269504088896341f
@@ -367,7 +367,7 @@ __device__ __forceinline__ float exp_from(float x, float m) { return x == -INFIN
 
 // NCH > 0: rows of up to NCH * 8 * KDT_NT elements are asked for before anything else and stay in registers.
 // One read of the logits, bound by HBM and, nearly, by its vector instructions (as the selection): 5000 bf16 rows of 30 522 with 64 kept
-// 70 us = 4.4 TB/s, 12 000 155 us = 4.7 TB/s; 330 rows 12 us.
+// 72 us = 4.2 TB/s, 12 000 155 us = 4.7 TB/s; 330 rows 11 us.
 template <typename T, bool REST, int NCH>
 __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void kd_top_fwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, const float* __restrict__ lse_t,
@@ -573,7 +573,7 @@ template <typename T> __device__ __forceinline__ void store8_past(T* p, const fl
 // Rows are taken from the last to the first: the forward sweep left the last ones in the 256 MB cache.  NT: a gradient that does not
 // fit into that cache is stored past it, and the logits stay (bf16, 30 522 classes, 5000 rows, both directions: 198 us; with
 // plain stores 207, first row first as well 213; 12 000 rows 453, 484, 488).  A smaller one is read from there by the next product.
-// Bound by HBM: 107 us alone for 610 MB (5.7 TB/s).
+// Bound by HBM: 106 us alone for 610 MB (5.8 TB/s).
 template <typename T, bool REST, bool NT>
 __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, int k, float inv_t, float coef,

@@ -482,7 +482,7 @@ template <typename T> __device__ __forceinline__ void fwd_outside(const PkArgs& 
 // forward, rows split over the waves: NW * 32 rows of one (sequence, chunk of heads), keys in shared blocks of BN.
 // Bound by MFMA and vector instructions in turn: the exponentials of a wave's scores (16 cycles each of 64) wait for its product and
 // the next product for them; two waves a SIMD overlap them in part.  6 causal sequences of 1 500 - 9 000, heads 32/8 of 128, bf16:
-// 915 us = 0.86 PF/s (MFMA busy 38 % of the cycles, vector 41 %); 128 rows and two blocks of 64 keys in flight spilled: 1 075 us.
+// 895 us = 0.88 PF/s (MFMA busy 40 % of the cycles, vector 41 %, 1.8 - 1.9 GHz); two blocks of 64 keys in flight spilled: 1 075 us.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BN>
 __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 512 ? 1 : 2) void pk_fwd_rows_kernel(PkArgs a) {
@@ -717,7 +717,7 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
 // backward, dQ: NW * 32 rows as in the forward (KS: 32 rows, every wave with keys of its own, the waves' sums joined at the end);
 // delta = dO.O of the block's rows is formed here and kept for dK / dV.  Two waves a SIMD; the joined one at head dim 128 is faster
 // with one and no spills (32 sequences of 8 queries and 500 keys, heads 16/4, both directions: 73 and 83 us).
-// Bound as the forward pass: 5 causal sequences of 1 000 - 5 000, heads 16/4 of 128, bf16 (193 GF): 235 us = 0.82 PF/s, MFMA busy 37 %.
+// Bound as the forward pass: 5 causal sequences of 1 000 - 5 000, heads 16/4 of 128, bf16 (193 GF): 234 us = 0.82 PF/s, MFMA busy 37 %.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BN, bool KS>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 128) ? 1 : 2) void pk_bwd_dq_kernel(PkArgs a) {
@@ -827,7 +827,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 12
 // VL: V is read from LDS as well.  At head dim 128 the two accumulators take 128 registers, K and V as columns 64, two blocks of
 // scores 32: without V two waves fit a SIMD, and they hide what one wave with all of it in registers (512) had to wait for.
 // One register too many is worse than either: a spill's reload waits for the loads of the next rows.
-// The same documents (257 GF): 355 us = 0.72 PF/s, MFMA busy 32 %, and 35 us for the join of 208 MB of parts (5.9 TB/s).
+// The same documents (257 GF): 345 us = 0.74 PF/s, MFMA busy 32 %, and 36 us for the join of 208 MB of parts (5.8 TB/s).
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int RG, bool VL>
 __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) void pk_bwd_dkv_kernel(PkArgs a) {
