@@ -108,8 +108,8 @@ __device__ __forceinline__ int block_count(int v, int* red) {
 // counting, (value, lower class first) making every element distinct - the result does not depend on the order of collection.
 // Rows with long ties at the bound (more candidates than the list holds) and rows with NaN or without a finite maximum get the
 // exact bound by bisection over the row, first of the value, then of the class among equals.
-// Bound by its vector instructions beside HBM: 8 elements cost 14 instructions for the maximum (which is kept) and 56 slots for the sum (an
-// exponential takes four); the candidates are collected by pieces of 8 first (one compare a piece), then one element a thread: with every
+// Bound by its vector instructions beside HBM: 8 elements cost 14 instructions for the maximum (which is kept) and 40 slots for the sum (an
+// exponential takes two); the candidates are collected by pieces of 8 first (one compare a piece), then one element a thread: with every
 // thread testing the 8 of its own pieces, a wave went through nearly all of them for two or three candidates.
 // 3000 bf16 rows of 30 522, k = 64: 44 us = 4.2 TB/s (56 before these three); 7 rows: 7.8 us, the phases of one row after the other.
 #define TOP_NT 512

@@ -480,7 +480,7 @@ template <typename T> __device__ __forceinline__ void fwd_outside(const PkArgs& 
 
 // ---------------------------------------------------------------------------------------------
 // forward, rows split over the waves: NW * 32 rows of one (sequence, chunk of heads), keys in shared blocks of BN.
-// Bound by MFMA and vector instructions in turn: the exponentials of a wave's scores (16 cycles each of 64) wait for its product and
+// Bound by MFMA and vector instructions in turn: the exponentials of a wave's scores wait for its product and
 // the next product for them; two waves a SIMD overlap them in part.  6 causal sequences of 1 500 - 9 000, heads 32/8 of 128, bf16:
 // 895 us = 0.88 PF/s (MFMA busy 40 % of the cycles, vector 41 %, 1.8 - 1.9 GHz); two blocks of 64 keys in flight spilled: 1 075 us.
 // ---------------------------------------------------------------------------------------------
