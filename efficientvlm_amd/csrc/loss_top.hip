@@ -350,8 +350,9 @@ extern "C" int evlm_top_logits(int dtype, const void* logits, int R, int C, int6
 // ---------------------------------------------------------------------------------------------
 #define KDT_NT 512
 // stats of a row, kept for the backward pass
-// (maximum and sum of the row; teacher's normaliser and mass; raw maximum and sum of what the sweep covered; rest's mass)
-enum { ST_MAX = 0, ST_SUM, ST_NORM, ST_MASS, ST_RAW_MAX, ST_SWEEP_SUM, ST_P_REST, ST_N };
+// (maximum and sum of the row; teacher's normaliser and mass; raw maximum and sum of what the sweep covered; M q_rest - p_rest, formed
+// in 64 bits: where student and teacher agree it is a small difference of two numbers close to each other)
+enum { ST_MAX = 0, ST_SUM, ST_NORM, ST_MASS, ST_RAW_MAX, ST_SWEEP_SUM, ST_SHARE, ST_N };
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
@@ -363,7 +364,6 @@ __device__ __forceinline__ double wave_max_f64(double v) {
   for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
   return v;
 }
-__device__ __forceinline__ float exp_from(float x, float m) { return x == -INFINITY ? 0.f : __expf(x - m); }   // exp(x - m), x <= m
 
 // NCH > 0: rows of up to NCH * 8 * KDT_NT elements are asked for before anything else and stay in registers.
 // One read of the logits, bound by HBM and, nearly, by its vector instructions (as the selection): 5000 bf16 rows of 30 522 with 64 kept
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
   // of 1: the k + 1 terms are formed in 64 bits (32 kept four digits of such a row's loss).
   // (Maximum, sum relative to it): a log-sum-exp in one number would lose the sum next to a maximum of the type's lowest value.
   const double t = (double)inv_t, m_sweep = (double)m * t;
-  double top = m_sweep, total = (double)sum;
+  double top = m_sweep, total = (double)sum, swept = total;  // swept: the sum of what the sweep covered, relative to top
   double yd[NE], zd[NE];
 #pragma unroll
   for (int i = 0; i < NE; ++i) { yd[i] = ci[i] >= 0 ? (double)y[i] * t : -INFINITY; zd[i] = ci[i] >= 0 ? (double)z[i] * t : -INFINITY; }
@@ -504,7 +504,8 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
 #pragma unroll
     for (int i = 0; i < NE; ++i)
       if (64 * i < k && first[i] && top != -INFINITY) sk += exp(yd[i] - top);
-    total = wave_sum_f64(sk) + (m_sweep == -INFINITY ? (sum != sum ? (double)sum : 0.0) : (double)sum * exp(m_sweep - top));
+    swept = m_sweep == -INFINITY ? (sum != sum ? (double)sum : 0.0) : (double)sum * exp(m_sweep - top);
+    total = wave_sum_f64(sk) + swept;
   }
   const double ls = log(total);
   double norm, mass, p_rest = 0.0, p[NE] = {};
@@ -540,7 +541,7 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
     if (REST && p_rest != 0.0) L += p_rest * (log(p_rest) - ((m_sweep - top) + (log((double)sum) - ls)));
     rowloss[r] = w * (float)L;
     st[ST_MAX] = (float)top; st[ST_SUM] = (float)total; st[ST_NORM] = (float)norm; st[ST_MASS] = (float)(mass + p_rest);
-    st[ST_RAW_MAX] = m; st[ST_SWEEP_SUM] = sum; st[ST_P_REST] = (float)p_rest;
+    st[ST_RAW_MAX] = m; st[ST_SWEEP_SUM] = sum; st[ST_SHARE] = (float)((mass + p_rest) * (swept / total) - p_rest);
   }
 }
 __global__ __launch_bounds__(1024) void kd_top_sum_kernel(const float* __restrict__ rowloss, int R, float coef, float* __restrict__ loss) {
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict_
   }
   // the others: f * exp((v - raw maximum) / T)
   const float c2 = inv_t * TOP_LOG2E, raw = st[ST_RAW_MAX], sweep = st[ST_SWEEP_SUM], base = raw == -INFINITY ? 0.f : raw;
-  const float share = REST ? mass * (exp_from(raw * inv_t, top) * sweep / total) - st[ST_P_REST] : mass;
+  const float share = REST ? st[ST_SHARE] : mass;
   const float f = REST && sweep == 0.f ? 0.f : g * share / sweep;               // (no class is left: nothing is written that stays)
   for (int c = tid; c < dchunks; c += KDT_NT) {
     float v[8];

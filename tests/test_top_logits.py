@@ -492,3 +492,29 @@ def test_together():
     for a, b in zip(got, torch.autograd.grad(ref, (dx, dW, dE))):
         # four products of up to 1201 terms in a row, each good to (terms) F of its largest sums
         assert (a.double().cpu() - b).norm() <= 4 * 1201 * F * b.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", [700, 40000])
+def test_gradient_of_a_rest_close_to_the_teachers(dtype, C):
+    """student and teacher agree on the mass outside the kept classes to a few parts in 10^5: the rest's gradient is that difference,
+    formed from terms that carry it (64 bits), not from two f32 numbers next to each other.  The other classes hold 0: their sum is a
+    whole number, exact, and every exponent among them 0, so what remains are a dozen f32 roundings of the result itself"""
+    R, k = 4, 3
+    s = torch.zeros(R, C, dtype=dtype, device="cuda")
+    c = torch.randint(0, C // 2, (R, k), generator=torch.Generator().manual_seed(1)).cuda().int() * 2 + torch.tensor([0, 1, 0], device="cuda").int()
+    c[:, 2] = C - 1
+    v = torch.tensor([[5.0, 3.5, 1.25]], device="cuda").repeat(R, 1)
+    s.scatter_(1, c.long(), v.to(dtype))
+    lse = torch.logsumexp(s.double(), 1)
+    for off in (3e-5, -1e-4, 4e-6):
+        l = (lse + off).float()
+        a = s.detach().requires_grad_()
+        g = torch.autograd.grad(ops.soft_cross_entropy_top(a, v, c, lse=l), a)[0].double().cpu()
+        p = torch.exp(v.double() - l.double()[:, None]).sum(1)
+        q_rest = torch.exp(-torch.logsumexp(s.double(), 1)) * (C - k)
+        want = ((q_rest - (1 - p)) / (C - k) / R).cpu()
+        kept = torch.zeros(R, C, dtype=torch.bool).scatter_(1, c.long().cpu(), True)
+        want = want[:, None].expand(R, C)[~kept]
+        assert ((g[~kept] - want).abs() <= ((2.0 ** -8 if dtype == BF16 else 0) + 16 * F) * want.abs()).all(), off
