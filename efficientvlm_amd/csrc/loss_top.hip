@@ -145,11 +145,12 @@ __device__ __forceinline__ float max8(const TopRaw8<bf16>& x) {
 // exp((v - m) / T) = 2^((v - m) c2), c2 = log2e / T
 __device__ __forceinline__ float exp_diff(float v, float m, float c2) { return __builtin_amdgcn_exp2f((v - m) * c2); }
 // Sums of it over a row: v c2 - m c2 in one fma, and the sum afterwards by what the rounding of m c2 left (tail), so that it is as exact as
-// with the difference first.  Where m c2 is out of range (a maximum of the type's lowest value), the difference first.
+// with the difference first.  That rounding is half a unit of m c2, at most 1/2 up to 2^24; from 2^31 on it alone would take the terms
+// out of range (a maximum of -1e10, as masks leave it), so beyond 2^24 the difference comes first.
 struct ExpSum {
   float m, c2, off;
   bool in_range;
-  __device__ __forceinline__ ExpSum(float m_, float c2_) : m(m_), c2(c2_), off(-m_ * c2_), in_range(fabsf(m_ * c2_) < 1e30f) {}
+  __device__ __forceinline__ ExpSum(float m_, float c2_) : m(m_), c2(c2_), off(-m_ * c2_), in_range(fabsf(m_ * c2_) <= 0x1p24f) {}
   __device__ __forceinline__ float tail() const { return in_range ? __builtin_amdgcn_exp2f(-fmaf(m, c2, off)) : 1.0f; }
   template <bool FAST> __device__ __forceinline__ float of(float v) const {
     return FAST ? __builtin_amdgcn_exp2f(fmaf(v, c2, off)) : exp_diff(v, m, c2);

@@ -518,3 +518,52 @@ def test_gradient_of_a_rest_close_to_the_teachers(dtype, C):
         kept = torch.zeros(R, C, dtype=torch.bool).scatter_(1, c.long().cpu(), True)
         want = want[:, None].expand(R, C)[~kept]
         assert ((g[~kept] - want).abs() <= ((2.0 ** -8 if dtype == BF16 else 0) + 16 * F) * want.abs()).all(), off
+
+
+# ---- large constants (masked classes that are finite) ---------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", [900, 40000])
+@pytest.mark.parametrize("value", [-1e9, -1e10, -1e12, -1e20, -1e29, 1e10, 1e25])
+def test_top_of_rows_at_a_masking_constant(dtype, C, value):
+    """the log-sum-exp of rows whose every class holds a large constant is constant / T + log C: finite, and not the constant itself"""
+    x = rows(4, C, dtype, seed=2, layout="plain").clone()
+    x[0] = value
+    x[1, 7:] = value
+    x[2, ::2] = value
+    for T in (1.0, 1.5, 0.7, 4.0):
+        check_top(x, 20, T)
+    check_top(rows(3, C, dtype, seed=3), 20, 1e-9)            # ordinary logits, exponents of the same size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", [900, 40000])
+@pytest.mark.parametrize("value", [-3e8, -1e10, -1e12, -1e20, -1e29, 1e10, 1e25])
+def test_rest_at_a_masking_constant(dtype, C, value):
+    """a student whose every class outside the kept ones holds one large constant: the loss is finite, the rest's gradient spread evenly
+    over those classes, the kept classes' as in the definition.  Every exponent that enters is a difference of equal numbers, of
+    numbers 1e8 apart, or of kept logits (all their size: e), so the errors are those of e"""
+    R, k = 3, 5
+    for T in (1.0, 1.5, 0.7):
+        s, v, c, l = pair(R, C, k, dtype, seed=11, T=T)
+        full = torch.full_like(s, value).scatter_(1, c.long(), s.gather(1, c.long()))
+        a = full.detach().requires_grad_()
+        loss = ops.soft_cross_entropy_top(a, v, c, lse=l, temperature=T)
+        g = torch.autograd.grad(loss, a)[0].double().cpu()
+        L, _, G, _ = want_loss(full, v, c, l, T, None)
+        u = 2.0 ** -8 if dtype == BF16 else F
+        assert abs(float(loss) - float(L)) <= 2.0 ** -17 * abs(float(L))
+        e = float(s.gather(1, c.long()).abs().max() + v.abs().max()) / T + float(l.abs().max()) + 8
+        y, z = s.gather(1, c.long()).double().cpu() / T, v.double().cpu() / T
+        p = torch.exp(z - l.double().cpu()[:, None])
+        q = torch.softmax(full.double().cpu() / T, 1).gather(1, c.long().cpu())
+        got, want = g.gather(1, c.long().cpu()), G.gather(1, c.long().cpu())
+        assert ((got - want).abs() <= u * want.abs() + 16 * F * e * (p + q) / T / R + 1e-30).all()
+        p_rest = 1 - p.sum(1)
+        share = ((1 - p_rest) if value > 0 else -p_rest) / (C - k) / T / R                 # mass q_rest - p_rest; value > 0: q_rest = 1
+        kept = torch.zeros(R, C, dtype=torch.bool).scatter_(1, c.long().cpu(), True)
+        share = share[:, None].expand(R, C)[~kept]
+        # (p_rest of f32 terms: 8 F e of their size 1; C / 512 + 16 terms of the sum in a row)
+        slack = 8 * F * e / (C - k) / T / R
+        assert ((g[~kept] - share).abs() <= (u + (C / 512 + 32) * F) * share.abs() + slack).all()
