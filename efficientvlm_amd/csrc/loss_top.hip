@@ -533,6 +533,10 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
     for (int i = 0; i < NE; ++i)
       if (64 * i < k && p[i] != 0.0) p[i] /= zs;
   }
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) any |= ci[i] >= 0;
+  if (!__any(any)) { mass = p_rest = 0.0; }                  // a row without entries takes no part, whatever it holds
   double L = 0.0;
 #pragma unroll
   for (int i = 0; i < NE; ++i)
@@ -589,7 +593,7 @@ __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict_
   const float w = roww ? roww[r] : 1.0f;
   const float* st = stats + r * ST_N;
   const int dchunks = (int)(ldd >> 3);                       // (ldd % 8 == 0, rows 16-byte aligned)
-  if (w == 0.f || (!REST && st[ST_NORM] == -INFINITY)) {     // (block-uniform) takes no part / no entries
+  if (w == 0.f || st[ST_MASS] == 0.f) {                      // (block-uniform) takes no part / no entries
     if (!acc) {
       const float zero[8] = {};
       for (int c = tid; c < dchunks; c += KDT_NT) store8<T>(d + 8 * (int64_t)c, zero);

@@ -567,3 +567,24 @@ def test_rest_at_a_masking_constant(dtype, C, value):
         # (p_rest of f32 terms: 8 F e of their size 1; C / 512 + 16 terms of the sum in a row)
         slack = 8 * F * e / (C - k) / T / R
         assert ((g[~kept] - share).abs() <= (u + (C / 512 + 32) * F) * share.abs() + slack).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", [300, 33000])
+@pytest.mark.parametrize("rest", [False, True])
+def test_a_row_without_entries_holds_anything(dtype, C, rest):
+    """with and without the rest: such a row adds nothing and has a zero gradient, the other rows' are those without it"""
+    s, v, c, l = pair(4, C, 6, dtype, seed=3, rest=rest)
+    s, v, c = s.clone(), v.clone(), c.clone()
+    c[1], c[2] = -1, C
+    want, wg = check_loss(s, v, c, l)
+    for broken in (math.nan, math.inf, -math.inf):
+        s[1], s[2, 5:] = broken, broken
+        v[1], v[2] = broken, broken
+        if rest:
+            l[1] = broken
+        a = s.detach().requires_grad_()
+        loss = ops.soft_cross_entropy_top(a, v, c, lse=l)
+        g, = torch.autograd.grad(loss, a)
+        assert torch.equal(loss, want) and torch.equal(g, wg) and not g[1:3].any()
