@@ -351,18 +351,16 @@ extern "C" int evlm_top_logits(int dtype, const void* logits, int R, int C, int6
 // ---------------------------------------------------------------------------------------------
 #define KDT_NT 512
 // stats of a row, kept for the backward pass
-// (maximum and sum of the row; teacher's normaliser and mass; raw maximum and sum of what the sweep covered; M q_rest - p_rest, formed
-// in 64 bits: where student and teacher agree it is a small difference of two numbers close to each other)
-enum { ST_MAX = 0, ST_SUM, ST_NORM, ST_MASS, ST_RAW_MAX, ST_SWEEP_SUM, ST_SHARE, ST_N };
+// (maximum of the row, not yet times 1 / T, and sum; the teacher's log-sum-exp - without one: the largest kept logit - and mass; maximum
+// and sum of what the sweep covered; M q_rest - p_rest, formed in 64 bits: where student and teacher agree it is a small difference
+// of two numbers close to each other - without a rest: the sum of the kept logits' exponentials)
+// Maxima are logits themselves, exact: the backward pass forms differences first, so logits far from zero lose nothing (a rounded
+// logit / T of 1e6 would be 2^-5 off, 3 % of the probability).
+enum { ST_TOP = 0, ST_SUM, ST_NORM, ST_MASS, ST_SWEEP_MAX, ST_SWEEP_SUM, ST_SHARE, ST_N };
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ double wave_max_f64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
   return v;
 }
 
@@ -486,6 +484,7 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
   // of 1: the k + 1 terms are formed in 64 bits (32 kept four digits of such a row's loss).
   // (Maximum, sum relative to it): a log-sum-exp in one number would lose the sum next to a maximum of the type's lowest value.
   const double t = (double)inv_t, m_sweep = (double)m * t;
+  float raw_top = m;
   double top = m_sweep, total = (double)sum, swept = total;  // swept: the sum of what the sweep covered, relative to top
   double yd[NE], zd[NE];
 #pragma unroll
@@ -499,9 +498,10 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
       first[i] = ci[i] >= 0;
       if (64 * i < k && dup)
         for (int e = 0; e < k; ++e) first[i] = first[i] && !(e < tid + 64 * i && cls[e] == ci[i]);
-      if (first[i]) top = fmax(top, yd[i]);
+      if (first[i]) raw_top = fmaxf(raw_top, y[i]);
     }
-    top = wave_max_f64(top);
+    raw_top = wave_max(raw_top);
+    top = (double)raw_top * t;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
       if (64 * i < k && first[i] && top != -INFINITY) sk += exp(yd[i] - top);
@@ -510,8 +510,10 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
   }
   const double ls = log(total);
   double norm, mass, p_rest = 0.0, p[NE] = {};
+  float kept_norm, kept_sum = 0.f;                           // what the backward pass reads: see ST_NORM, ST_SHARE
   if constexpr (REST) {
-    norm = (double)lse_t[r];
+    kept_norm = lse_t[r];
+    norm = (double)kept_norm;
     mass = 0.0;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
@@ -519,14 +521,18 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
     mass = wave_sum_f64(mass);
     p_rest = mass != mass ? mass : (sum == 0.f ? 0.0 : fmax(0.0, 1.0 - mass));   // (sum == 0: no class is left for the rest)
   } else {
-    double zm = -INFINITY, zs = 0.0;
+    double zs = 0.0;
+    kept_norm = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) zm = fmax(zm, zd[i]);
-    zm = wave_max_f64(zm);
+    for (int i = 0; i < NE; ++i)
+      if (ci[i] >= 0) kept_norm = fmaxf(kept_norm, z[i]);
+    kept_norm = wave_max(kept_norm);
+    const double zm = (double)kept_norm * t;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
       if (64 * i < k && zd[i] != -INFINITY) { p[i] = exp(zd[i] - zm); zs += p[i]; }
     zs = wave_sum_f64(zs);
+    kept_sum = (float)zs;
     norm = zm == -INFINITY ? -INFINITY : zm + log(zs);
     mass = zm == -INFINITY ? (zs != zs ? zs : 0.0) : (zs != zs ? zs : 1.0);
 #pragma unroll
@@ -545,8 +551,8 @@ __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void k
   if (tid == 0) {
     if (REST && p_rest != 0.0) L += p_rest * (log(p_rest) - ((m_sweep - top) + (log((double)sum) - ls)));
     rowloss[r] = w * (float)L;
-    st[ST_MAX] = (float)top; st[ST_SUM] = (float)total; st[ST_NORM] = (float)norm; st[ST_MASS] = (float)(mass + p_rest);
-    st[ST_RAW_MAX] = m; st[ST_SWEEP_SUM] = sum; st[ST_SHARE] = (float)((mass + p_rest) * (swept / total) - p_rest);
+    st[ST_TOP] = raw_top; st[ST_SUM] = (float)total; st[ST_NORM] = kept_norm; st[ST_MASS] = (float)(mass + p_rest);
+    st[ST_SWEEP_MAX] = m; st[ST_SWEEP_SUM] = sum; st[ST_SHARE] = REST ? (float)((mass + p_rest) * (swept / total) - p_rest) : kept_sum;
   }
 }
 __global__ __launch_bounds__(1024) void kd_top_sum_kernel(const float* __restrict__ rowloss, int R, float coef, float* __restrict__ loss) {
@@ -601,18 +607,18 @@ __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict_
     return;
   }
   const float g = gout[0] * coef * w * inv_t;
-  const float top = st[ST_MAX], total = st[ST_SUM], mass = st[ST_MASS], norm = st[ST_NORM];
+  const float top = st[ST_TOP], total = st[ST_SUM], mass = st[ST_MASS], norm = st[ST_NORM];
   const T* x = s + r * ld;
   int ci = -1;
   float y = 0.f, before = 0.f;
   if (tid < k) {
     ci = classes[r * k + tid];
     if (ci < 0 || ci >= C) ci = -1;
-    const float z = ci >= 0 ? values[r * k + tid] * inv_t : -INFINITY;
+    const float z = ci >= 0 ? values[r * k + tid] : -INFINITY;
     cls[tid] = ci;
-    prob[tid] = z == -INFINITY ? 0.f : expf(z - norm);
+    prob[tid] = z == -INFINITY ? 0.f : (REST ? expf(fmaf(z, inv_t, -norm)) : expf((z - norm) * inv_t) / st[ST_SHARE]);
     if (ci >= 0) {
-      y = to_f(x[ci]) * inv_t;
+      y = to_f(x[ci]);
       if (acc) before = to_f(d[ci]);
     }
   }
@@ -621,10 +627,10 @@ __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict_
   if (ci >= 0) {
     float p = 0.f;
     for (int j = 0; j < k; ++j) p += cls[j] == ci ? prob[j] : 0.f;
-    mine = g * (mass * (expf(y - top) / total) - p) + before;
+    mine = g * (mass * (expf((y - top) * inv_t) / total) - p) + before;
   }
   // the others: f * exp((v - raw maximum) / T)
-  const float c2 = inv_t * TOP_LOG2E, raw = st[ST_RAW_MAX], sweep = st[ST_SWEEP_SUM], base = raw == -INFINITY ? 0.f : raw;
+  const float c2 = inv_t * TOP_LOG2E, raw = st[ST_SWEEP_MAX], sweep = st[ST_SWEEP_SUM], base = raw == -INFINITY ? 0.f : raw;
   const float share = REST ? st[ST_SHARE] : mass;
   const float f = REST && sweep == 0.f ? 0.f : g * share / sweep;               // (no class is left: nothing is written that stays)
   for (int c = tid; c < dchunks; c += KDT_NT) {

@@ -588,3 +588,41 @@ def test_a_row_without_entries_holds_anything(dtype, C, rest):
         loss = ops.soft_cross_entropy_top(a, v, c, lse=l)
         g, = torch.autograd.grad(loss, a)
         assert torch.equal(loss, want) and torch.equal(g, wg) and not g[1:3].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("size", [3e3, 1e5, 1e6])
+def test_gradient_of_logits_far_from_zero(rest, size):
+    """logits around +-size, a few units apart: every probability is an exponent of differences (exact in f32), so the gradient is as good as
+    around zero.  (logits times the f32 1 / T, rounded before the difference, would be off by size 2^-24: 6 % of a probability at 1e6)"""
+    R, C, k, T = 6, 200, 9, 0.7
+    g = torch.Generator().manual_seed(4)
+    # whole multiples of 2^-4: f32 holds them up to 2^20
+    t = (torch.randn(R, C, generator=g) * 32).round() / 16
+    s = (t * 16 + (torch.randn(R, C, generator=g) * 8).round()).round() / 16
+    inv = float(torch.tensor(1.0 / T, dtype=F32))
+    for shift in (size, -size):
+        shift = float(round(shift))
+        x, y = (s + shift).cuda(), (t + shift).cuda()
+        v, c, _ = ops.top_logits(y, k)
+        # a log-sum-exp of the teacher as f32 holds it; rows in which it leaves the kept classes more than all mass have no rest
+        l = torch.logsumexp(y.double() * inv, 1).float() if rest else None
+        a = x.detach().requires_grad_()
+        got = torch.autograd.grad(ops.soft_cross_entropy_top(a, v, c, lse=l, temperature=T), a)[0].double().cpu()
+        xs, at = s.double() * inv, c.long().cpu()
+        q = torch.softmax(xs, 1)
+        z = v.double().cpu() * inv
+        p = torch.softmax(z, 1) if l is None else torch.exp(z - l.double().cpu()[:, None])
+        P = torch.zeros_like(q).scatter_(1, at, p)
+        if rest:
+            kept = torch.zeros_like(q, dtype=torch.bool).scatter_(1, at, True)
+            p_rest = (1 - p.sum(1, keepdim=True)).clamp_min(0)
+            mass = p.sum(1, keepdim=True) + p_rest
+            q_rest = q.masked_fill(kept, 0).sum(1, keepdim=True)
+            want = torch.where(kept, mass * q - P, q / q_rest * (mass * q_rest - p_rest))
+        else:
+            want = q - P
+        # exponents up to e = (spread of the logits) / T: 4 F e each; sums of C terms; p_rest of 64-bit terms
+        e = 2 * float((s.max() - s.min()).clamp_min(float(t.max() - t.min()))) * inv + 16
+        assert ((got - want / T / R).abs() <= 8 * F * e * (q + P) * (1.5 if not rest else 3) / T / R + 4 * F * want.abs() + 1e-12).all()
