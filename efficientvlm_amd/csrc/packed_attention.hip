@@ -677,31 +677,30 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
   if (inside && c.n == 1) return;
   T* o = (T*)a.out + ((int64_t)t * a.H + h) * a.dh;
   float M = -INFINITY, L = 0.f, v0 = 0.f, v1 = 0.f;
-  if (inside) {
+  const int vis = inside ? vis_of(a, c.q, t - c.q.qs) : 0;
+  if (vis > 0) {                                             // (a maximum of -inf is no row without keys: its scores may all be NaN)
     const int unit = h / a.gp, r = (t - c.q.qs - c.tile * a.per) * a.gp + h % a.gp;      // (heads of a unit are consecutive)
     const int n = __builtin_amdgcn_readfirstlane((int)min((int64_t)c.n, a.tiles - c.first));                             // (never past the workspace)
     for (int i = lane; i < n; i += 64) M = fmaxf(M, part_of(a, c.first + i, unit)[32 * a.dh + 2 * r]);
     M = wave_max(M);
-    if (M != -INFINITY) {
-      const unsigned d0 = min(lane, a.dh - 1), d1 = min(lane + 64, a.dh - 1);
-      const int64_t next = (int64_t)a.units * (32 * (a.dh + 2));
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        float f = 0.f;
-        if (i0 + lane < n) {
-          const float* ml = part_of(a, c.first + i0 + lane, unit) + 32 * a.dh + 2 * r;
-          f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[0] - M) * a.c);
-          L = fmaf(ml[1], f, L);
-        }
-        const int e = min(64, n - i0);
-        const float* p = (const float*)uniform64((int64_t)(part_of(a, c.first + i0, unit) + r * a.dh));
-        int i = 0;
-        for (; i + 8 <= e; i += 8) join_parts<8>(p + i * next, next, 8, d0, d1, f, i, v0, v1);
-        for (; i < e; i += 4) join_parts<4>(p + i * next, next, e - i, d0, d1, f, i, v0, v1);
+    const unsigned d0 = min(lane, a.dh - 1), d1 = min(lane + 64, a.dh - 1);
+    const int64_t next = (int64_t)a.units * (32 * (a.dh + 2));
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      float f = 0.f;
+      if (i0 + lane < n) {
+        const float* ml = part_of(a, c.first + i0 + lane, unit) + 32 * a.dh + 2 * r;
+        f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[0] - M) * a.c);
+        L = fmaf(ml[1], f, L);
       }
-      L = wave_sum(L);
+      const int e = min(64, n - i0);
+      const float* p = (const float*)uniform64((int64_t)(part_of(a, c.first + i0, unit) + r * a.dh));
+      int i = 0;
+      for (; i + 8 <= e; i += 8) join_parts<8>(p + i * next, next, 8, d0, d1, f, i, v0, v1);
+      for (; i < e; i += 4) join_parts<4>(p + i * next, next, e - i, d0, d1, f, i, v0, v1);
     }
+    L = wave_sum(L);
   }
-  const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+  const float inv = vis > 0 ? 1.0f / L : 0.f;
   v0 *= inv; v1 *= inv;
   if (lane < a.dh) o[lane] = from_f<T>(v0);
   if (lane + 64 < a.dh) o[lane + 64] = from_f<T>(v1);
@@ -710,7 +709,7 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
     if (lane < a.dh) lo[lane] = from_f<T>(v0 - to_f(from_f<T>(v0)));
     if (lane + 64 < a.dh) lo[lane + 64] = from_f<T>(v1 - to_f(from_f<T>(v1)));
   }
-  if (a.lse && lane == 0) a.lse[(int64_t)h * a.Tq + t] = M == -INFINITY ? INFINITY : fmaf(M, a.c, __builtin_amdgcn_logf(L));
+  if (a.lse && lane == 0) a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(M, a.c, __builtin_amdgcn_logf(L)) : INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------

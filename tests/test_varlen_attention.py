@@ -503,3 +503,35 @@ def test_keys_behind_two_to_the_31():
     val, tol = definition(p["q"], p["k"], p["k"], None, p["q0"], p["lq"], p["k0"], p["lk"], True, dh ** -0.5, 2.0 ** -8)
     check([got], val, tol)
     check([want], val, tol)
+
+
+# ---- broken values, large scores, wide strides -------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,dh", [((8, 2), 64), ((4, 4), 128)])
+def test_a_broken_query_shows_however_long_its_cache(dtype, heads, dh):
+    """a NaN in one head's query, NaN in every key, or every score -inf: NaN in exactly the rows of those heads, whether the keys are
+    one piece (short caches) or joined from several"""
+    for lk in ([20, 33, 5], [3000, 1700, 2000]):
+        p = problem(dtype, *heads, dh, [1, 2, 1], lk, slots=5)
+        G, b, m = heads[0] // heads[1], p["k0"][1], p["lk"][1]
+        for kind in ("query", "keys", "far"):
+            clean, q, k = p["q"].clone(), p["q"].clone(), p["k"].clone()
+            bad = [(t, h) for t in (1, 2) for h in range(G)]
+            if kind == "query":
+                q[2, 1, 3] = math.nan
+                bad = [(2, 1)]
+            elif kind == "keys":
+                k[b:b + m, 0] = math.nan
+            else:
+                clean = q = q.abs() + 0.1
+                k[b:b + m, 0] = -math.inf
+            got = run({**p, "q": q, "k": k})
+            broken = torch.zeros(got[0].shape[:2], dtype=torch.bool, device="cuda")
+            for t, h in bad:
+                broken[t, h] = True
+            assert got[0][broken].isnan().all() and got[1][broken].isnan().all(), (kind, lk)
+            val, tol = definition(clean, p["k"], p["v"], p["dout"], p["q0"], p["lq"], p["k0"], p["lk"], True, dh ** -0.5,
+                                  2.0 ** -8 if dtype == BF16 else F)
+            good = ~broken.cpu()
+            check([x[~broken] for x in got[:2]], [x[good] for x in val[:2]], [x[good] for x in tol[:2]])
