@@ -1524,23 +1524,23 @@ def _same_device(first, *others):
             raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
 
 
-def _heads3(x):
-    """x [tokens, heads, dh] as the packed kernels read it: heads in whole 16-byte pieces, 16-byte aligned, strides below 2^22
+def _heads3(x, keys=False):
+    """x [tokens, heads, dh] as the packed kernels read it: heads in whole 16-byte pieces, 16-byte aligned, the token stride - of
+    queries the head stride, too; `keys`' heads may lie any distance apart, as in a cache stored [heads, tokens, dh] - below 2^22
     elements (slices of a packed projection are; anything else is copied).  Returns (tensor, address, token stride, head stride)."""
     mask = 7 if x.dtype == torch.bfloat16 else 3
-    for _ in range(2):
-        n, h, _d = x.shape
-        st, sh, sd = x.stride()
-        st, sh, p = st if n > 1 else 0, sh if h > 1 else 0, x.data_ptr()
-        if sd == 1 and not ((st | sh) & mask or p & 15 or max(st, sh) >= 1 << 22):
-            break
+    n, h, d = x.shape
+    st, sh, sd = x.stride()
+    st, sh, p = st if n > 1 else 0, sh if h > 1 else 0, x.data_ptr()
+    if sd != 1 or (st | sh) & mask or p & 15 or (st if keys else max(st, sh)) >= 1 << 22:
         x = x.clone(memory_format=torch.contiguous_format)
+        st, sh, p = h * d if n > 1 else 0, d if h > 1 else 0, x.data_ptr()
     return x, p, st, sh
 
 
 def _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal):
     """(args, tensors the pointers in them belong to) of one packed-attention launch"""
-    (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = _heads3(q), _heads3(k), _heads3(v)
+    (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = _heads3(q), _heads3(k, True), _heads3(v, True)
     Tq, H, dh = q.shape
     a = L.PackedAttnArgs(L.BF16 if q.dtype == torch.bfloat16 else L.F32, Tq, k.shape[0], cu_q.shape[0] - 1, H, k.shape[1], dh,
                          causal, scale, qp, kp, vp, qt, qh, kt, kh, vt, vh, cu_q.data_ptr(), cu_k.data_ptr(),

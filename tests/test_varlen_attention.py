@@ -535,3 +535,52 @@ def test_a_broken_query_shows_however_long_its_cache(dtype, heads, dh):
                                   2.0 ** -8 if dtype == BF16 else F)
             good = ~broken.cpu()
             check([x[~broken] for x in got[:2]], [x[good] for x in val[:2]], [x[good] for x in tol[:2]])
+
+
+def test_wide_head_strides_of_keys_are_read_in_place():
+    """a cache stored [heads, tokens, dh] has heads 2^22 and more elements apart; only the token stride of K and V is limited, and both
+    strides of Q and dO"""
+    wide = torch.empty_strided((10, 2, 128), (128, 1 << 22, 1), dtype=BF16)
+    x, address, token, head = ops._heads3(wide, keys=True)
+    assert x is wide and address == wide.data_ptr() and (token, head) == (128, 1 << 22)
+    x, address, token, head = ops._heads3(wide)
+    assert x.is_contiguous() and address == x.data_ptr() != wide.data_ptr() and (token, head) == (256, 128)
+    apart = torch.empty_strided((2, 2, 128), (1 << 22, 128, 1), dtype=BF16)
+    for keys in (False, True):
+        x, address, token, head = ops._heads3(apart, keys=keys)
+        assert x.is_contiguous() and address == x.data_ptr() != apart.data_ptr() and (token, head) == (256, 128)
+    one = apart[:1]                                           # (a single token has no stride)
+    assert ops._heads3(one)[1] == one.data_ptr()
+    odd = torch.empty(10, 2, 129, dtype=BF16)[..., 1:]
+    for keys in (False, True):
+        assert ops._heads3(odd, keys=keys)[0].is_contiguous()
+    many = torch.empty(2, 1 << 15, 129, dtype=BF16)[..., 1:]  # 2^15 heads of 128: a token stride of 2^22 however it is laid out (the
+    x, address, token, head = ops._heads3(many)               # entry refuses it); the address is that of the tensor that is kept
+    assert address == x.data_ptr() and (token, head) == (1 << 22, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lq", [[1, 1], [70, 300]])
+def test_heads_first_caches_of_any_length(dtype, lq):
+    """K and V with heads 2^22 elements apart: the values of packed ones"""
+    p = problem(dtype, 8, 2, 128, lq, [900, 1400])
+    tokens = (1 << 15) + 64
+    far = {}
+    for n in "kv":
+        store = torch.zeros(2, tokens, 128, dtype=dtype, device="cuda")
+        store[:, :2300] = p[n].transpose(0, 1)
+        far[n] = store.transpose(0, 1)
+    with torch.no_grad():
+        out = ops.packed_attention(p["q"], far["k"], far["v"], p["cu_q"], p["cu_k"])
+    val, tol = definition(p["q"], p["k"], p["v"], None, p["q0"], p["lq"], p["k0"], p["lk"], True, 128 ** -0.5,
+                          2.0 ** -8 if dtype == BF16 else F)
+    check([out], val, tol)
+    if lq[0] > 1:
+        q, k, v = (t.detach().requires_grad_() for t in (p["q"], far["k"], far["v"]))
+        out = ops.packed_attention(q, k, v, p["cu_q"], p["cu_k"])
+        got = torch.autograd.grad(out, (q, k, v), p["dout"])
+        val, tol = definition(p["q"], p["k"], p["v"], p["dout"], p["q0"], p["lq"], p["k0"], p["lk"], True, 128 ** -0.5,
+                              2.0 ** -8 if dtype == BF16 else F)
+        check((out, got[0], got[1][:2300], got[2][:2300]), val, tol)
+        assert not got[1][2300:].any() and not got[2][2300:].any()
