@@ -745,7 +745,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 12
   const int64_t t = q.qs + tok;
   typename TL::frag qf[TL::NS], df[TL::NS];
   TL::load_cols(valid ? (const T*)a.Q + t * a.q_tok + h * a.q_head : nullptr, a.dh, hh, qf);
-  TL::load_cols(valid ? (const T*)a.dO + t * a.do_tok + h * a.do_head : nullptr, a.dh, hh, df);
+  TL::load_cols(vis > 0 ? (const T*)a.dO + t * a.do_tok + h * a.do_head : nullptr, a.dh, hh, df);      // (a row that sees no key: 0 whatever its dO)
   float delta = 0.f;
   {
     typename TL::frag of[TL::NS];

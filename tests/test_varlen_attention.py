@@ -584,3 +584,24 @@ def test_heads_first_caches_of_any_length(dtype, lq):
                               2.0 ** -8 if dtype == BF16 else F)
         check((out, got[0], got[1][:2300], got[2][:2300]), val, tol)
         assert not got[1][2300:].any() and not got[2][2300:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lq,lk", [([9, 5], [4, 2]), ([200, 140], [150, 30])])
+@pytest.mark.parametrize("broken", [math.nan, math.inf])
+def test_rows_that_see_no_key_hold_anything(dtype, lq, lk, broken):
+    """causal, more queries than keys: the first queries of a sequence see nothing.  Their output and their gradient are zero and nothing
+    of them enters another gradient, whatever stands in their queries and in the gradient of their output"""
+    for heads in ((4, 4), (6, 2)):
+        p = problem(dtype, *heads, 64, lq, lk)
+        want = run(p)
+        q, dout = p["q"].clone(), p["dout"].clone()
+        blind = torch.zeros(q.shape[0], dtype=torch.bool, device="cuda")
+        for a, n, m in zip(p["q0"], lq, lk):
+            blind[a:a + n - m] = True
+        q[blind], dout[blind] = broken, broken
+        got = run({**p, "q": q, "dout": dout})
+        assert (got[0][blind] == 0).all() and (got[1][blind] == 0).all()
+        for g, w in zip(got, want):
+            assert torch.equal(g, w)
