@@ -70,7 +70,7 @@ class XAttnFusedArgs(C.Structure):
 
 class PackedAttnArgs(C.Structure):
     _fields_ = [("dtype", _i), ("Tq", _i), ("Tk", _i), ("S", _i), ("H", _i), ("Hkv", _i), ("dh", _i), ("causal", _i),
-                ("scale", _f), ("Q", _vp), ("K", _vp), ("V", _vp),
+                ("scale", _f), ("lse_planes", _i), ("Q", _vp), ("K", _vp), ("V", _vp),
                 ("q_tok", _i64), ("q_head", _i64), ("k_tok", _i64), ("k_head", _i64), ("v_tok", _i64), ("v_head", _i64),
                 ("cu_q", _vp), ("cu_k", _vp), ("k_lens", _vp), ("O", _vp), ("O_lo", _vp), ("lse", _vp), ("workspace", _vp),
                 ("dO", _vp), ("dQ", _vp), ("dK", _vp), ("dV", _vp),

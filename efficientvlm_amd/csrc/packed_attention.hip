@@ -8,6 +8,9 @@
 //   dP_j = dO.v_j,  delta = dO.O = sum_j p_j dP_j,  dS_j = p_j (dP_j - delta)
 //   dQ = scale sum_j dS_j k_j,   dK_j = scale sum_rows dS_j q,   dV_j = sum_rows p_j dO   (rows of every head of the group)
 //   A row that sees no key has O = 0 and adds nothing to any gradient.
+//   A row whose largest score m is far from zero, |m c| > 2^10 with c = scale log2e, has its exponents formed as (s_j - m) c - log2 sum_j
+//   2^((s_j - m) c) instead: s_j c - lse would carry the rounding of m c or of lse, half a unit of numbers of that size.  (Scores of
+//   3e5: probabilities of the backward pass 1 % off; from 3e9 on out of f32's range, NaN.  Up to 2^10 it is 2^-15.)
 //
 // All four products of a step are built from two wave-level forms over 32 x 32 blocks:
 //   row_mm   C[r][c] = sum_d tile[r][d] col[c][d]     tile rows from LDS, columns held in registers for the whole loop
@@ -27,6 +30,7 @@
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 #define PK_LOG2E 1.44269504088896341f
+#define PK_FAR 1024.0f
 
 struct PkArgs {
   const void *Q, *K, *V, *O, *dO;
@@ -37,6 +41,7 @@ struct PkArgs {
   int Tq, Tk, S, H, G, dh;          // G = heads per key head
   int gp, chunks, units;            // heads packed into a row block, chunks of a group, chunks * key heads
   int per, tiles;                   // tokens (keys) of a block, grid tiles
+  int far;                          // lse has a second plane, for the rows far from zero
   int splits, causal;               // splits: parts of the rows of a key block (dK / dV)
   int want;                         // chunks of keys aimed at for one chunk of heads (forward, few rows)
   unsigned inv_gp;                  // 2^16 / gp rounded up: r / gp = r * inv_gp >> 16 for r < 256
@@ -415,7 +420,8 @@ __device__ __forceinline__ void attend(const char* Ks, const char* Vs, int kt0, 
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
   mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
   const float mn = fmaxf(m, mx);
-  if (__any((mn - m) * c > 8.0f)) {
+  float mc = m == -INFINITY ? 0.f : m * c;
+  if (__any((mn - m) * c > 8.0f || fabsf(mc) > PK_FAR)) {
     const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
     m = mn;
     l *= alpha;
@@ -423,8 +429,16 @@ __device__ __forceinline__ void attend(const char* Ks, const char* Vs, int kt0, 
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+    mc = m == -INFINITY ? 0.f : m * c;
+    if (__any(fabsf(mc) > PK_FAR)) {
+      const float base = fabsf(mc) > PK_FAR ? m : 0.f;
+      mc = fabsf(mc) > PK_FAR ? 0.f : mc;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] -= base;
+    }
   }
-  const float mc = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -463,6 +477,21 @@ template <typename T, int D> __device__ __forceinline__ void store_rest(T* row, 
         Vec4<T>::store(row + d, v);
       }
     }
+}
+// a row's log-sum-exp for the backward pass, from its maximum and its sum relative to it.  A row far from zero keeps its maximum in the
+// second plane, and the log of that sum so that it shows: (log + 1) 2^100, where the others are at most 2^11
+__device__ __forceinline__ void store_lse(const PkArgs& a, int h, int64_t t, float m, float l, int vis) {
+  const int64_t at = (int64_t)h * a.Tq + t;
+  const float logl = __builtin_amdgcn_logf(l);
+  const bool far = a.far && vis > 0 && fabsf(m * a.c) > PK_FAR;
+  a.lse[at] = vis > 0 ? (far ? (logl + 1.0f) * 0x1p100f : fmaf(m, a.c, logl)) : INFINITY;
+  if (far) a.lse[(int64_t)a.H * a.Tq + at] = m;
+}
+// ... read: the maximum of a row far from zero (and its lse relative to it), 0 for any other
+__device__ __forceinline__ float far_base(const PkArgs& a, int64_t at, float& lse) {
+  if (!(a.far && fabsf(lse) > 0x1p64f && fabsf(lse) < INFINITY)) return 0.f;
+  lse = lse * 0x1p-100f - 1.0f;
+  return a.lse[(int64_t)a.H * a.Tq + at];
 }
 template <typename T> __device__ __forceinline__ void zero_row(T* row, int dh) {
   for (int d = threadIdx.x & 63; d < dh; d += 64) row[d] = from_f<T>(0.f);
@@ -523,7 +552,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 512 ? 1 : 2) void pk_fwd_
   const float inv = vis > 0 ? 1.0f / l : 0.f;
   store_cols<T, D>((T*)a.out + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
   if (sizeof(T) == 2 && a.out_lo) store_rest<T, D>((T*)a.out_lo + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
-  if (a.lse && hh == 0) a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(m, a.c, __builtin_amdgcn_logf(l)) : INFINITY;
+  if (a.lse && hh == 0) store_lse(a, h, t, m, l, vis);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -638,7 +667,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void pk_fwd_keys_k
       if (!whole) {
         part[32 * a.dh + 2 * r] = M; part[32 * a.dh + 2 * r + 1] = L;
       } else if (a.lse) {
-        a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(M, a.c, __builtin_amdgcn_logf(L)) : INFINITY;
+        store_lse(a, h, t, M, L, vis);
       }
     }
   } else {
@@ -646,7 +675,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) void pk_fwd_keys_k
     const float inv = vis > 0 ? 1.0f / l : 0.f;
     store_cols<T, D>((T*)a.out + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
     if (sizeof(T) == 2 && a.out_lo) store_rest<T, D>((T*)a.out_lo + (t * a.H + h) * a.dh, a.dh, o, inv, hh);
-    if (a.lse && hh == 0) a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(m, a.c, __builtin_amdgcn_logf(l)) : INFINITY;
+    if (a.lse && hh == 0) store_lse(a, h, t, m, l, vis);
   }
 }
 
@@ -709,7 +738,7 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
     if (lane < a.dh) lo[lane] = from_f<T>(v0 - to_f(from_f<T>(v0)));
     if (lane + 64 < a.dh) lo[lane + 64] = from_f<T>(v1 - to_f(from_f<T>(v1)));
   }
-  if (a.lse && lane == 0) a.lse[(int64_t)h * a.Tq + t] = vis > 0 ? fmaf(M, a.c, __builtin_amdgcn_logf(L)) : INFINITY;
+  if (a.lse && lane == 0) store_lse(a, h, t, M, L, vis);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -764,7 +793,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 12
     delta += __shfl_xor(delta, 32, 64);
     if (valid && hh == 0 && own == 0) a.delta[(int64_t)h * a.Tq + t] = delta;
   }
-  const float lse = valid ? a.lse[(int64_t)h * a.Tq + t] : INFINITY;
+  float lse = valid ? a.lse[(int64_t)h * a.Tq + t] : INFINITY;
+  const float base = far_base(a, (int64_t)h * a.Tq + t, lse);
+  const bool far = __any(base != 0.f);
   const T* Kb = (const T*)a.K + q.ks * a.k_tok + kh * a.k_head;
   const T* Vb = (const T*)a.V + q.ks * a.v_tok + kh * a.v_head;
   f32x16 acc[D / 32] = {};
@@ -784,9 +815,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 12
       for (int b = 0; b < BN / 32; ++b) {
         f32x16 s = TL::row_mm(Ks, 32 * b, qf, lane);
         const f32x16 dp = TL::row_mm(Vs, 32 * b, df, lane);
-        if (mask) {
+        if (mask | far) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = kt + 32 * b + c_row(i, hh) < vis ? s[i] : -INFINITY;
+          for (int i = 0; i < 16; ++i) s[i] = kt + 32 * b + c_row(i, hh) < vis ? s[i] - base : -INFINITY;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * (dp[i] - delta);
@@ -834,8 +865,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) v
   constexpr int BR = 32 * RG, KG = NW / RG, JOIN = KG * (RG - 1) * 32 * D * 4;
   constexpr int VB = VL ? KG * 32 * TL::RB : 0, SM = VB + 2 * BR * TL::RB > JOIN ? VB + 2 * BR * TL::RB : JOIN;
   __shared__ __attribute__((aligned(512))) char sm[SM];
-  __shared__ __attribute__((aligned(16))) float Ls[BR], Ds[BR];
+  __shared__ __attribute__((aligned(16))) float Ls[BR], Ds[BR], Bs[BR];
   __shared__ __attribute__((aligned(16))) int Vis[BR];
+  __shared__ int Far[RG];                                    // does any of 32 rows have a base?
   char *Vs = sm, *Qs = sm + VB, *Os = Qs + BR * TL::RB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, kg = wave / RG, rg = wave % RG;
   const int nkh = a.H / a.G, kh = blockIdx.x % nkh;
@@ -867,7 +899,6 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) v
   int ch = per_chunk ? b0 / per_chunk : 0, tok0 = first + (b0 - ch * per_chunk) * btok;
   Stage<T, D, BR, 64 * NW> qs, os;
   float lv = INFINITY, dl = 0.f;
-  int vi = 0;
   auto load = [&](int c, int t0) {
     const int h0 = kh * a.G + c * a.gp;
     qs.load_rows((const T*)a.Q + q.qs * a.q_tok + h0 * a.q_head, a.q_tok, a.q_head, t0, q.qlen, a.gp, a.inv_gp, a.dh, tid);
@@ -878,7 +909,6 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) v
       const int64_t at = (int64_t)(h0 + tid - rt * a.gp) * a.Tq + q.qs + tok;
       lv = in ? a.lse[at] : INFINITY;
       dl = in ? a.delta[at] : 0.f;
-      vi = in ? vis_of(a, q, tok) : 0;
     }
   };
   if (b0 < b1) load(ch, tok0);
@@ -886,8 +916,15 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) v
     __syncthreads();
     qs.pad(a.dh, tid); os.pad(a.dh, tid);
     qs.store(Qs, tid); os.store(Os, tid);
-    if (tid < BR) { Ls[tid] = lv; Ds[tid] = dl; Vis[tid] = vi; }
+    if (tid < BR) {
+      const int rt = (int)(tid * a.inv_gp >> 16), tok = tok0 + rt;
+      const float bs = far_base(a, (int64_t)(kh * a.G + ch * a.gp + tid - rt * a.gp) * a.Tq + q.qs + tok, lv);
+      Ls[tid] = lv; Ds[tid] = dl; Bs[tid] = bs; Vis[tid] = tid < used && tok < q.qlen ? vis_of(a, q, tok) : 0;
+      const unsigned long long any = __ballot(bs != 0.f);
+      if ((tid & 31) == 0) Far[tid >> 5] = (uint32_t)(any >> (tid & 32)) != 0u;
+    }
     __syncthreads();
+    const bool far = __builtin_amdgcn_readfirstlane(Far[rg]) != 0;      // (asked for ahead of the products, whose reads cover it)
     const int now = tok0;
     tok0 += btok;
     if (tok0 >= q.qlen) { tok0 = first; ++ch; }
@@ -901,6 +938,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) v
     f32x16 p = TL::template row_mm<VL>(Qs, r_lo, kf, lane), ds;
     if constexpr (VL) ds = TL::row_mm(Os, r_lo, Vs, w0 - k0, lane);
     else ds = TL::row_mm(Os, r_lo, vf, lane);
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] -= Bs[r_lo + c_row(i, hh)];
+    }
     if (mask) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = key < Vis[r_lo + c_row(i, hh)] ? p[i] : -INFINITY;
@@ -1063,6 +1104,7 @@ static int pk_check(const evlm_packed_attn_args* x, const char* name) {
 static PkArgs pk_args(const evlm_packed_attn_args* x) {
   PkArgs a = {};
   a.Q = x->Q; a.K = x->K; a.V = x->V; a.out = x->O; a.O = x->O; a.out_lo = x->O_lo; a.lse = x->lse;
+  a.far = x->lse_planes == 2;
   a.cu_q = x->cu_q; a.cu_k = x->cu_k; a.k_lens = x->k_lens;
   a.q_tok = x->q_tok; a.q_head = x->q_head; a.k_tok = x->k_tok; a.k_head = x->k_head; a.v_tok = x->v_tok; a.v_head = x->v_head;
   a.Tq = x->Tq; a.Tk = x->Tk; a.S = x->S; a.H = x->H; a.G = x->H / x->Hkv; a.dh = x->dh;

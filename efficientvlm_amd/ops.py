@@ -1543,7 +1543,7 @@ def _packed_args(q, k, v, cu_q, cu_k, k_lens, scale, causal):
     (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = _heads3(q), _heads3(k, True), _heads3(v, True)
     Tq, H, dh = q.shape
     a = L.PackedAttnArgs(L.BF16 if q.dtype == torch.bfloat16 else L.F32, Tq, k.shape[0], cu_q.shape[0] - 1, H, k.shape[1], dh,
-                         causal, scale, qp, kp, vp, qt, qh, kt, kh, vt, vh, cu_q.data_ptr(), cu_k.data_ptr(),
+                         causal, scale, 2, qp, kp, vp, qt, qh, kt, kh, vt, vh, cu_q.data_ptr(), cu_k.data_ptr(),
                          None if k_lens is None else k_lens.data_ptr())
     return a, (q, k, v)
 
@@ -1560,7 +1560,7 @@ class _PackedAttention(torch.autograd.Function):
             lo = lse = ws = None
             a.O = O.data_ptr()
             if need:
-                lse = q.new_empty((H, Tq), dtype=torch.float32)
+                lse = q.new_empty((2, H, Tq), dtype=torch.float32)
                 a.lse = lse.data_ptr()
                 if q.dtype == torch.bfloat16:                   # (what rounding takes from O)
                     lo = torch.empty_like(O)
@@ -1586,7 +1586,7 @@ class _PackedAttention(torch.autograd.Function):
             dq = q.new_empty(q.shape)
             # (the kernels write every key of every sequence and the rows outside all of them; unfilled room is left alone)
             dk, dv = (k.new_empty(k.shape), v.new_empty(k.shape)) if k_lens is None else (k.new_zeros(k.shape), v.new_zeros(k.shape))
-            delta = torch.empty_like(lse)
+            delta = torch.empty_like(lse[0])
             a.O, a.lse, a.delta, a.dQ, a.dK, a.dV = O.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
             if lo is not None:
                 a.O_lo = lo.data_ptr()

@@ -298,7 +298,9 @@ int evlm_copy_few(const void* const* src, void* const* dst, const int64_t* nbyte
  *   captured launch serves every batch of the same Tq, Tk, S.  Starts and lengths are clamped to the tensors.
  *   causal: query i of n sees keys j < m - n + i + 1 of m (the last query sees all).  A row that sees no key, and a row outside
  *   all sequences, has O = 0; so have the gradients of keys that no row sees.
- *   lse [H, Tq] f32 (forward: written if given; backward: as the forward wrote it).  delta [H, Tq] f32: backward scratch.
+ *   lse [H, Tq] f32 (forward: written if given; backward: as the forward wrote it).  With lse_planes 2 it is [2, H, Tq]: rows whose largest
+ *   score m has |scale m log2e| > 2^10 keep m in the second plane (the others 0) and an lse relative to it; without it, the gradients of
+ *   such rows carry an error of about |scale m| 2^-24 relative to themselves.  delta [H, Tq] f32: backward scratch.
  *   workspace: evlm_packed_attention_workspace() floats, uninitialised, for one call at a time.
  * The decoder side of the reference pads its answers to the longest (eff_bert.py:317-355 over [B, L] rows, the causal mask of
  * :975-996); packed rows do the same arithmetic without the padding.
@@ -308,6 +310,7 @@ typedef struct {
   int Tq, Tk, S, H, Hkv, dh;
   int causal;
   float scale;                  /* > 0 */
+  int lse_planes;               /* 2: lse is [2, H, Tq], see above; anything else (the word was padding once): [H, Tq] */
   const void* Q; const void* K; const void* V;
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
   const int32_t* cu_q; const int32_t* cu_k; const int32_t* k_lens;

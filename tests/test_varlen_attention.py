@@ -605,3 +605,50 @@ def test_rows_that_see_no_key_hold_anything(dtype, lq, lk, broken):
         assert (got[0][blind] == 0).all() and (got[1][blind] == 0).all()
         for g, w in zip(got, want):
             assert torch.equal(g, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [1e3, 3e5, 2e7, 3e9, 1e13, 1e25])
+@pytest.mark.parametrize("heads,dh,lq,lk", [
+    ((4, 4), 64, [3, 9, 1], None), ((4, 2), 64, [300, 130], None), ((4, 2), 128, [300, 130], None), ((8, 2), 64, [1, 2], [3000, 1700]),
+    ((2, 2), 64, [40, 30], [500, 300]), ((4, 4), 128, [3, 9, 1], None), ((2, 2), 128, [40, 30], [500, 300])])
+def test_scores_of_any_size(dtype, size, heads, dh, lq, lk):
+    """scores far from zero and far apart (products of powers of two: exact): each row's weight lies on its largest visible key, or in
+    halves on two that are equal.  O and dV are those of one or two terms; dS is p (dP - delta), the difference of two sums of dh terms"""
+    H, Hkv = heads
+    p = problem(dtype, H, Hkv, dh, lq, lk, seed=8)
+    g = torch.Generator().manual_seed(9)
+    q, k = torch.zeros(p["q"].shape), torch.zeros(p["k"].shape)
+    unit = 2.0 ** math.floor(math.log2(size) / 2)
+    for sign in (1.0, -1.0):
+        q[..., 5] = unit
+        # heights 1 .. 1.75 in steps of 1/8 (bf16 holds them): 32 keys in a row meet each height several times
+        height = torch.randint(0, 7, k.shape[:2], generator=g)
+        k[..., 5] = sign * unit * (1 + height / 8.0)
+        pp = {**p, "q": q.to(dtype).cuda(), "k": k.to(dtype).cuda()}
+        got = [t.double().cpu() for t in run(pp, scale=1.0)]
+        u = 2.0 ** -8 if dtype == BF16 else F
+        V, dO, K = p["v"].double().cpu(), p["dout"].double().cpu(), k.double()
+        val, eV = [torch.zeros_like(x) for x in got], torch.zeros_like(V)
+        for a, n, b, m in zip(p["q0"], p["lq"], p["k0"], p["lk"]):
+            seen = torch.arange(m)[None, :] <= torch.arange(n)[:, None] + (m - n)
+            for h in range(H):
+                at, rows, kh = slice(b, b + m), slice(a, a + n), h // (H // Hkv)
+                P = torch.softmax((K[at, kh, 5] * unit).expand(n, m).masked_fill(~seen, -math.inf), 1)
+                val[0][rows, h] = P @ V[at, kh]
+                dP = dO[rows, h] @ V[at, kh].T
+                dS = P * (dP - (dP * P).sum(1, keepdim=True))
+                val[1][rows, h] = dS @ K[at, kh]
+                val[2][at, kh] += dS.T @ q[rows, h].double()
+                val[3][at, kh] += P.T @ dO[rows, h]
+                eV[at, kh] += P.sum(0)[:, None]               # rows that lie on the key
+        # p: the scores are exact; a row's sum has up to m equal terms, (m + 16) F, and p is rounded to u as an operand.  Below 2^10 a score
+        # of log2 e times that size is itself rounded, by 2^-15, up to four times (m, its share in the sums of two waves, the log-sum-exp)
+        rel = (max(p["lk"]) + 16) * F + u + (2.0 ** -13 if size < 1e4 else 0.0)
+        D = 2 * (dO.abs().amax(2).max() * V.abs().sum(2).max())                    # at least |dP| + |delta|
+        count = (H // Hkv) * max(p["lq"]) + 16
+        tol = [rel * V.abs().max(), (rel + u + 4 * (dh + 16) * F) * D * 2 * unit, (rel + u + (4 * (dh + 16) + count) * F) * D * unit * eV,
+               (rel + count * F) * dO.abs().max() * eV]
+        for x, w, t, name in zip(got, val, tol, ("O", "dQ", "dK", "dV")):
+            assert ((x - w).abs() <= u * w.abs() + t + 1e-30).all(), (name, size, sign)
