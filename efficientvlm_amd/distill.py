@@ -9,6 +9,7 @@ import os
 import torch
 
 from . import ops
+from .runtime import branch_stream
 
 
 def get_cor_teacher(teacher_reps, student_reps, is_attn=False):
@@ -221,9 +222,6 @@ def vqa_loss_mix(loss_small, kd, lagrangian, kd_corr=None):
                                                               loss_kd=loss_kd)
 
 
-_SIDE = {}
-
-
 def _tensors(obj):
     if torch.is_tensor(obj):
         yield obj
@@ -259,10 +257,7 @@ def student_and_teacher(student_call, teacher_call, ref_tensor, overlap):
     stream (joined before returning) so that it shares the chip with the student forward"""
     if overlap and ref_tensor.is_cuda:
         cur = torch.cuda.current_stream()
-        dev = ref_tensor.device
-        side = _SIDE.get(dev)
-        if side is None:
-            side = _SIDE[dev] = torch.cuda.Stream(device=dev)
+        side = branch_stream("teacher", ref_tensor.device)
         side.wait_stream(cur)
         with torch.cuda.stream(side), torch.no_grad():
             T = teacher_call()

@@ -30,6 +30,32 @@ def compute(dtype):
         _STATE["dtype"] = old
 
 
+_BRANCHES = {}          # (device index, role) -> stream
+_RING = 32              # torch hands out side streams in turn from a pool of this size
+
+
+def branch_stream(role, device=None, draw=None):
+    """The side stream of `role` ("capture", "text", "teacher", ...): one per role and device in the process, no two of them the same
+    hardware stream.  torch.cuda.Stream() takes the next of a ring of 32, so streams that are drawn on their own coincide as soon
+    as a program has drawn others in between; two branches of one hipGraph capture that do run as one nested fork, which this
+    stack does not survive (a segmentation fault in hipGraphLaunch).  Every stream that a trainer captures on, forks into or
+    exchanges gradients on comes from here.  `draw` makes a stream of `device` (tests)."""
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
+    stream = _BRANCHES.get((index, role))
+    if stream is None:
+        taken = {s.cuda_stream for (i, _), s in _BRANCHES.items() if i == index}
+        for _ in range(2 * _RING):
+            stream = draw(index) if draw is not None else torch.cuda.Stream(device=index)
+            if stream.cuda_stream not in taken:
+                break
+        else:
+            raise RuntimeError(f"no side stream of its own for '{role}': every one of the pool is taken by {len(taken)} others")
+        _BRANCHES[index, role] = stream
+    return stream
+
+
 COLLECTIVES = None      # tests: set to a list -> every collective of a step is appended as (kind, numel, dtype)
 
 

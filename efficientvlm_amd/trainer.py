@@ -25,7 +25,7 @@ import torch.distributed as dist
 
 from . import distill, ops
 from .optim import FlatAdamW
-from .runtime import compute, log_collective
+from .runtime import branch_stream, compute, log_collective
 
 
 def dist_ready():
@@ -113,7 +113,7 @@ class GradReducer:
         self.buckets = self._buckets(self.flat)
         # (a high-priority stream was measured - profiles/r05_exchange_overlap.md: it gets a hardware queue of its own, and a
         # long kernel on it then starves every normal-priority queue: 24.7 against 17.9 ms in the simulated-wire probe)
-        self.stream = torch.cuda.Stream() if (self.flat and self.flat[0].is_cuda) else None
+        self.stream = branch_stream("exchange", self.flat[0].device) if (self.flat and self.flat[0].is_cuda) else None
         self._pending = []
         self.coalesce = self.active and self._probe_coalescing()
         self.launch = "coalesced" if self.coalesce else "per-range"
@@ -326,7 +326,7 @@ class _StagedExchange:
         if cur != torch.cuda.default_stream():
             return fn()
         if getattr(self, "_loop", None) is None:
-            self._loop = torch.cuda.Stream()
+            self._loop = branch_stream("loop")
         self._loop.wait_stream(cur)
         with torch.cuda.stream(self._loop):
             out = fn()
@@ -477,7 +477,7 @@ class GDTrainer(_StagedExchange):
         # gradient stage relies on every text-side gradient being issued before backward enters the image encoder)
         if (hasattr(student, "text_stream") and not self.reducer.active and not os.environ.get("EVLM_NO_TEXT_STREAM")
                 and next(student.parameters()).is_cuda):
-            student.text_stream = torch.cuda.Stream()
+            student.text_stream = branch_stream("text")
         self.use_graph = use_graph
         self.wgrad_inplace = True
         if not os.environ.get("EVLM_TEACHER_ALL_MAPS"):
@@ -501,7 +501,7 @@ class GDTrainer(_StagedExchange):
         self.out = None
         self._graphs = {}
         self._pipes, self._pending = {}, None
-        self._side = torch.cuda.Stream() if next(student.parameters()).is_cuda else None
+        self._side = branch_stream("teacher") if next(student.parameters()).is_cuda else None
         self._tpool = self._spool = None
         self._joint = {}
         if self.world > 1:
@@ -610,7 +610,7 @@ class GDTrainer(_StagedExchange):
         state = [(g["m"].clone(), g["v"].clone()) for g in self.opt.groups], self.opt.step_count
         cur = torch.cuda.current_stream()
         self._keep_ST = True
-        warm = torch.cuda.Stream()                         # warm-up on a side stream, as torch.cuda.graph asks for
+        warm = branch_stream("warm")                       # warm-up on a side stream, as torch.cuda.graph asks for
         warm.wait_stream(cur)
         with torch.cuda.stream(warm):
             for _ in range(2):
@@ -783,7 +783,7 @@ class GDTrainer(_StagedExchange):
                 ops.CACHE.invalidate()                             # capture the casts of the trainable weights too
                 ops.reserve_tables()
                 g = torch.cuda.CUDAGraph()
-                with no_gc_during_capture(), torch.cuda.graph(g, pool=self._spool):
+                with no_gc_during_capture(), torch.cuda.graph(g, pool=self._spool, stream=branch_stream("capture")):
                     res = self._joint_body(pipe, p, pp, pk)
                 ops.flush_table_uploads()
                 self._spool = g.pool()
@@ -839,7 +839,7 @@ class GDTrainer(_StagedExchange):
         stream in the segment behind the ITC gather and joins where that segment ends"""
         from .efficient_models import xvlm as X
         if self._cap_stream is None:
-            self._cap_stream, self._seg_pool = torch.cuda.Stream(), torch.cuda.graph_pool_handle()
+            self._cap_stream, self._seg_pool = branch_stream("capture"), torch.cuda.graph_pool_handle()
         cur, cs, side = torch.cuda.current_stream(), self._cap_stream, self._side
         ops.reserve_tables()
         torch.cuda.synchronize()
@@ -1100,7 +1100,7 @@ class GDTrainer(_StagedExchange):
     def _capture(self, batch):
         static = {k: v.clone() for k, v in batch.items()}
         state = [(g["m"].clone(), g["v"].clone()) for g in self.opt.groups], self.opt.step_count
-        side = torch.cuda.Stream()
+        side = branch_stream("warm")
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for _ in range(2):                             # warm-up on a side stream (allocator + weight caches);
@@ -1113,7 +1113,7 @@ class GDTrainer(_StagedExchange):
         self.opt.set_schedule(0.0)                         # (the captured optimiser step reads the staged scalars at replay)
         graph = torch.cuda.CUDAGraph()
         pool = next(iter(self._graphs.values()))[0].pool() if self._graphs else None   # the kinds never run concurrently
-        with no_gc_during_capture(), torch.cuda.graph(graph, pool=pool):
+        with no_gc_during_capture(), torch.cuda.graph(graph, pool=pool, stream=branch_stream("capture")):
             out = self._step_eager(static)
         ops.flush_table_uploads()
         # the warm-up advanced Adam's step count and moments: restore them so replay k is optimiser step k
@@ -1141,7 +1141,7 @@ class TeacherPrefetch:
     def __init__(self, run_teacher, use_graph=True):
         self.run_teacher = run_teacher          # fn(batch dict) -> teacher outputs (any nest of tensors)
         self.use_graph = use_graph
-        self.side = torch.cuda.Stream()
+        self.side = branch_stream("prefetch")
         self.states, self.pending, self.last_key = {}, None, None
         self._tick = 0
 
@@ -1268,7 +1268,7 @@ class _CapturedStep:
         if self.reducer.active or not os.environ.get("EVLM_L0_STREAM") or not self._pruned_dev.is_cuda:
             return None
         if getattr(self, "_l0_stream", None) is None:
-            self._l0_stream = torch.cuda.Stream()
+            self._l0_stream = branch_stream("l0")
         cur, ls = torch.cuda.current_stream(), self._l0_stream
         ls.wait_stream(cur)
         with torch.cuda.stream(ls):
@@ -1355,7 +1355,7 @@ class _CapturedStep:
         # a non-capturing stream into the graph (hipGraphInstantiate then faults on this stack)
         cur = torch.cuda.current_stream()
         if self._cap_stream is None:
-            self._cap_stream = torch.cuda.Stream()
+            self._cap_stream = branch_stream("capture")
         cs = self._cap_stream
         kind = tuple(key[2:])
         ent = self._sgraphs.get(key)
