@@ -652,3 +652,76 @@ def test_scores_of_any_size(dtype, size, heads, dh, lq, lk):
                (rel + count * F) * dO.abs().max() * eV]
         for x, w, t, name in zip(got, val, tol, ("O", "dQ", "dK", "dV")):
             assert ((x - w).abs() <= u * w.abs() + t + 1e-30).all(), (name, size, sign)
+
+
+# ---- nothing beyond the tensors ------------------------------------------------------------------------
+GUARD = 1 << 14
+
+
+class Guarded:
+    """buffers of exactly the size that a C entry is told, between two zones that have to stay as they are"""
+
+    def __init__(self):
+        self.all = []
+
+    def __call__(self, shape, dtype, fill=None):
+        n = math.prod(shape) * torch.empty(0, dtype=dtype).element_size()
+        buf = torch.full((n + 2 * GUARD,), 0x5A, dtype=torch.uint8, device="cuda")
+        self.all.append(buf)
+        view = buf[GUARD:GUARD + n].view(dtype).view(shape)
+        if fill is not None:
+            view.copy_(fill)
+        return view
+
+    def intact(self):
+        return all((b[:GUARD] == 0x5A).all() and (b[-GUARD:] == 0x5A).all() for b in self.all)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Tq,Tk,S,heads,dh,chunked,split", [
+    (20, 20, 2, (4, 4), 64, False, False), (3, 6000, 3, (8, 2), 64, True, False), (5, 5000, 2, (4, 4), 128, True, False),
+    (1500, 300, 1, (8, 1), 64, False, True), (1600, 900, 1, (12, 2), 128, False, True), (700, 900, 70, (6, 2), 24, False, False)])
+def test_no_starts_make_a_kernel_leave_its_tensors(dtype, Tq, Tk, S, heads, dh, chunked, split):
+    """starts and lengths of any content, through the C entries: outputs, statistics and workspaces lie between zones that stay as
+    they were.  Scores of any size, with one and two planes of lse"""
+    from efficientvlm_amd import _lib
+    lib = _lib.load()
+    H, Hkv = heads
+    g = torch.Generator().manual_seed(Tq + S)
+    even = lambda T: [T * i // S for i in range(S + 1)]
+    wild = lambda n, T: torch.where(torch.rand(n, generator=g) < 0.3, torch.randint(-2 ** 31, 2 ** 31 - 1, (n,), generator=g),
+                                    torch.randint(-9, T + 9, (n,), generator=g)).tolist()
+    cases = [(even(Tq), even(Tk), None, 1.0), (even(Tq), even(Tk), wild(S, Tk), 1e6), (even(Tq), even(Tk), None, 1e12),
+             ([2 ** 31 - 1, -2 ** 31] * S, [5, -7] * S, None, 1.0), ([0] + [Tq] * S, [Tk] * S + [0], None, 1.0)]
+    cases += [(wild(S + 1, Tq), wild(S + 1, Tk), wild(S, Tk) if i % 2 else None, 1.0) for i in range(6)]
+    for i, (cu_q, cu_k, k_lens, size) in enumerate(cases):
+        print(f"case {i}", flush=True)
+        i32 = lambda x: None if x is None else torch.tensor(x[:S + 1], dtype=torch.int32, device="cuda")
+        cu_q, cu_k, k_lens = i32(cu_q), i32(cu_k), i32(k_lens)
+        new = Guarded()
+        planes = 1 + i % 2
+        r = lambda *s: torch.randn(*s, generator=g) * size
+        q, k, v, dout = (new(s, dtype, r(*s)) for s in ((Tq, H, dh), (Tk, Hkv, dh), (Tk, Hkv, dh), (Tq, H, dh)))
+        out, lo, dq = (new((Tq, H, dh), dtype) for _ in range(3))
+        dk, dv = (new((Tk, Hkv, dh), dtype) for _ in range(2))
+        lse, delta = new((planes, H, Tq), F32), new((H, Tq), F32)
+        a = _lib.PackedAttnArgs(dtype=_lib.BF16 if dtype == BF16 else _lib.F32, Tq=Tq, Tk=Tk, S=S, H=H, Hkv=Hkv, dh=dh, causal=i % 3 != 2,
+                                scale=dh ** -0.5, lse_planes=planes, Q=q.data_ptr(), K=k.data_ptr(), V=v.data_ptr(),
+                                q_tok=H * dh, q_head=dh, k_tok=Hkv * dh, k_head=dh, v_tok=Hkv * dh, v_head=dh, cu_q=cu_q.data_ptr(),
+                                cu_k=cu_k.data_ptr(), k_lens=None if k_lens is None else k_lens.data_ptr(), O=out.data_ptr(),
+                                O_lo=lo.data_ptr(), lse=lse.data_ptr(), dO=dout.data_ptr(), dQ=dq.data_ptr(), dK=dk.data_ptr(),
+                                dV=dv.data_ptr(), do_tok=H * dh, do_head=dh, dq_tok=H * dh, dq_head=dh, dk_tok=Hkv * dh, dk_head=dh,
+                                dv_tok=Hkv * dh, dv_head=dh, delta=delta.data_ptr())
+        for backward, entry in ((0, lib.evlm_packed_attention_fwd), (1, lib.evlm_packed_attention_bwd)):
+            n = lib.evlm_packed_attention_workspace(ctypes.byref(a), backward)
+            assert (n > 0) == (split if backward else chunked)
+            a.workspace = new((n,), F32).data_ptr() if n else None
+            assert entry(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert new.intact(), i
+        if i == 0:
+            at = lambda c: c[:-1].tolist()
+            n = lambda c: (c[1:] - c[:-1]).tolist()
+            val, tol = definition(q, k, v, dout, at(cu_q), n(cu_q), at(cu_k), n(cu_k), True, dh ** -0.5, 2.0 ** -8 if dtype == BF16 else F)
+            check((out, dq, dk, dv), val, tol)
