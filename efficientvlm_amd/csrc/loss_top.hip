@@ -366,7 +366,7 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 
 // NCH > 0: rows of up to NCH * 8 * KDT_NT elements are asked for before anything else and stay in registers.
 // One read of the logits, bound by HBM and, nearly, by its vector instructions (as the selection): 5000 bf16 rows of 30 522 with 64 kept
-// 72 us = 4.2 TB/s, 12 000 155 us = 4.7 TB/s; 330 rows 11 us.
+// 76 us = 4.0 TB/s (median of 23, shortest 73), 12 000 155 us = 4.7 TB/s; 330 rows 11 us.
 template <typename T, bool REST, int NCH>
 __global__ __launch_bounds__(KDT_NT, sizeof(T) == 2 ? (REST ? 8 : 6) : 4) void kd_top_fwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, const float* __restrict__ lse_t,
@@ -585,7 +585,7 @@ template <typename T> __device__ __forceinline__ void store8_past(T* p, const fl
 // Rows are taken from the last to the first: the forward sweep left the last ones in the 256 MB cache.  NT: a gradient that does not
 // fit into that cache is stored past it, and the logits stay (bf16, 30 522 classes, 5000 rows, both directions: 198 us; with
 // plain stores 207, first row first as well 213; 12 000 rows 453, 484, 488).  A smaller one is read from there by the next product.
-// Bound by HBM: 106 us alone for 610 MB (5.8 TB/s).
+// Bound by HBM: 118 us for 610 MB (5.2 TB/s; median of 23, the shortest 106).
 template <typename T, bool REST, bool NT>
 __global__ __launch_bounds__(KDT_NT) void kd_top_bwd_kernel(const T* __restrict__ s, int C, int64_t ld, const float* __restrict__ values,
                                                             const int32_t* __restrict__ classes, int k, float inv_t, float coef,

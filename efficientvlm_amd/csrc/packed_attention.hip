@@ -94,8 +94,8 @@ template <typename T, int D> struct Tile {
     }
   }
   // order of a product's LDS reads and MFMAs: the reads of the next two steps on their way before a step's products.  (Left alone, the
-  // compiler reuses one step's registers and waits for every read; most of that wait is hidden by the SIMD's other wave: the
-  // documents' backward pass 605 -> 594 us, 9 000-token prompts 908 -> 892; one step 602 / 902, three 605 / 899.)
+  // compiler reuses one step's registers and waits for every read; most of that wait is hidden by the SIMD's other wave.  Left alone,
+  // one, two, three steps: the documents below, both directions, 777, 767, 762, 773 us; the prompts' forward 899, 900, 889, 893.)
   template <int READS, int N> static __device__ __forceinline__ void ahead() {
     constexpr int AHEAD = 2;
     if constexpr (sizeof(T) == 2) {
@@ -399,7 +399,10 @@ template <typename T, int D, int ROWS, int NT> struct Stage {
 // one block of NB * 32 keys for 32 rows: scores, running maximum, probabilities, context.  m is kept as a raw score; it follows
 // the true maximum only when that has grown by more than 2^8 (p then stays <= 2^8, far from any overflow of the f32 sums, and
 // bf16 keeps the same relative precision), so the rescaling of the context is rare.  p is rounded to bf16 for the second
-// product (its sum is not): half a step of 2^-8 relative to each p.
+// product (its sum is not): half a step, 2^-8 relative to each p (a product in f32 has a sixteenth of the rate, p as a sum of two bf16
+// would cost it twice).  The backward pass rounds p and dS = p (dP - delta) likewise, as operands of dV, dK and dQ.  The products of inputs that are bf16 already
+// are exact in f32, so these are the only roundings beside the outputs': errors against 64 bits are 1.1 - 1.5 x those of a form in
+// f32 that rounds its outputs alone (1.1 for short rows, whose p are few; 1.5 for the gradients of short sequences).
 template <typename T, int D, int NB>
 __device__ __forceinline__ void attend(const char* Ks, const char* Vs, int kt0, int vis, bool mask,
                                        const typename Frag<T>::type (&qf)[Tile<T, D>::NS], float c, float& m, float& l,
@@ -509,9 +512,11 @@ template <typename T> __device__ __forceinline__ void fwd_outside(const PkArgs& 
 
 // ---------------------------------------------------------------------------------------------
 // forward, rows split over the waves: NW * 32 rows of one (sequence, chunk of heads), keys in shared blocks of BN.
-// Bound by MFMA and vector instructions in turn: the exponentials of a wave's scores wait for its product and
-// the next product for them; two waves a SIMD overlap them in part.  6 causal sequences of 1 500 - 9 000, heads 32/8 of 128, bf16:
-// 895 us = 0.88 PF/s (MFMA busy 40 % of the cycles, vector 41 %, 1.8 - 1.9 GHz); two blocks of 64 keys in flight spilled: 1 075 us.
+// 6 causal sequences of 1 653 - 4 965 (22 492 tokens), heads 32/8 of 128, bf16: 890 us = 0.89 PF/s.  No unit is the bound by itself: MFMA are busy
+// 39 % of the cycles, vector instructions 40 % (1.8 - 1.9 GHz); of the waves' cycles 21 % wait for memory, LDS and barriers, 41 % for their
+// turn to issue.  Within a wave the exponentials of its scores wait for the product and the next product for them, and two waves a
+// SIMD overlap that in part: a loop without the maximum, a quarter fewer vector instructions, took the same time, so it is the
+// chain and not the instructions' number.  Two blocks of 64 keys in flight a wave spilled: 1 075 us.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BN>
 __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 512 ? 1 : 2) void pk_fwd_rows_kernel(PkArgs a) {
@@ -745,7 +750,11 @@ template <typename T> __global__ __launch_bounds__(256) void pk_join_kernel(PkAr
 // backward, dQ: NW * 32 rows as in the forward (KS: 32 rows, every wave with keys of its own, the waves' sums joined at the end);
 // delta = dO.O of the block's rows is formed here and kept for dK / dV.  Two waves a SIMD; the joined one at head dim 128 is faster
 // with one and no spills (32 sequences of 8 queries and 500 keys, heads 16/4, both directions: 73 and 83 us).
-// Bound as the forward pass: 5 causal sequences of 1 000 - 5 000, heads 16/4 of 128, bf16 (193 GF): 234 us = 0.82 PF/s, MFMA busy 37 %.
+// 5 causal sequences of 1 148 - 4 956 (10 156 tokens), heads 16/4 of 128, bf16 (193 GF): 247 us = 0.78 PF/s (median of 23, shortest 235), MFMA busy
+// 38 % of the cycles at 2.0 GHz.  45 % of the waves' cycles are waits: one buffer of keys between two barriers a step, filled through
+// registers.
+// Spills at bf16, head dim 128 (256 registers): 2 of the 128-row form, each half of a step reads one again; 59 of the one-wave form, 8 reads a
+// step - it still is the faster one for short sequences (171 us, 224 with 128-row blocks, below).
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BN, bool KS>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 128) ? 1 : 2) void pk_bwd_dq_kernel(PkArgs a) {
@@ -856,8 +865,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 || (KS && NW > 1 && D == 12
 // a key block and leave f32 parts (joined by pk_bwd_join_kernel) where there are few key blocks.
 // VL: V is read from LDS as well.  At head dim 128 the two accumulators take 128 registers, K and V as columns 64, two blocks of
 // scores 32: without V two waves fit a SIMD, and they hide what one wave with all of it in registers (512) had to wait for.
-// One register too many is worse than either: a spill's reload waits for the loads of the next rows.
-// The same documents (257 GF): 345 us = 0.74 PF/s, MFMA busy 32 %, and 36 us for the join of 208 MB of parts (5.8 TB/s).
+// One register too many is worse than either: a spill's reload waits for the loads of the next rows (base of rows far from zero kept in a
+// register between the loads and the barrier: 3 spilled, 768 us for the documents' both directions; read where it is needed: 753).
+// The same documents (257 GF): 376 us = 0.68 PF/s (median of 23, shortest 354), MFMA busy 33 % at 2.0 GHz, 46 % of the waves' cycles waits, and
+// 36 us for the join of 208 MB of parts (5.8 TB/s).  The one-wave form at bf16, head dim 128 spills 13 registers beside 512 in use.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int RG, bool VL>
 __global__ __launch_bounds__(64 * NW, sizeof(T) * D == 128 || NW == 8 ? 2 : 1) void pk_bwd_dkv_kernel(PkArgs a) {
@@ -1159,6 +1170,8 @@ template <typename T, int D> static int pk_fwd_launch(PkArgs& a, bool few, int64
   return 0;
 }
 
+// Head dims run the code of the next of 64 and 128, the pieces behind them zero: 32 pays for products and LDS of 64 (20 causal sequences of
+// 42 - 884, heads 12/4, both directions: 89 us, 95 at 64), 72 - 120 for those of 128.
 #define PK_DISPATCH(x, CALL)                                                                                   \
   ((x)->dtype == EVLM_BF16 ? ((x)->dh <= 64 ? CALL<bf16, 64> : CALL<bf16, 128>)                                \
                            : ((x)->dh <= 64 ? CALL<float, 64> : CALL<float, 128>))

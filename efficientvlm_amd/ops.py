@@ -1613,8 +1613,9 @@ def packed_attention(q, k, v, cu_q, cu_k=None, k_lens=None, scale=None, causal=T
     launch follows their contents.
     causal: query i of n sees keys j < m - n + i + 1 of m, so the last query sees every key (a whole prompt, a chunk behind a
     cache, a single new token).  scale: 1 / sqrt(dh) unless given, positive.
-    A row that sees no key, and a row outside all sequences, is zero; gradients likewise.  Within one sequence, keys that
-    causality hides from a row must hold finite values (their probability is an exact 0, 0 * inf is not).
+    A row that sees no key, and a row outside all sequences, is zero; gradients likewise, whatever they hold.  Within one sequence,
+    keys that causality hides from a row, and the gradients of outputs that see a key, must hold finite values (their probability
+    is an exact 0, 0 * inf is not); a NaN in a query, or in a key that it sees, is NaN in that row's output.
 
     The padded kinds are self_attention / cross_attention (with the probability map as an output); the decoder masks of
     eff_bert.py:975-996 are the causal form here."""
@@ -2671,7 +2672,8 @@ def soft_cross_entropy_top(predicts, values, classes, lse=None, temperature=1.0,
     row_weight [...] (default 1) times KL(p || softmax(predicts / temperature)), a device scalar:
       lse None:  p = softmax(values / temperature) over the kept classes (the teacher renormalised);
       lse [...]: p = exp(values / temperature - lse), lse being the teacher's log-sum-exp at the SAME temperature; the mass that
-                 is not kept counts as one more class, against the student's mass on the classes that are not kept.
+                 is not kept counts as one more class, against the student's mass on the classes that are not kept (where it has
+                 none at all - every one of them -inf, or none left - that class takes no part).
     Entries whose class lies outside 0 .. C-1 take no part (padding of rows that kept fewer; -1 by custom); a row without
     entries, and a row of weight 0, adds nothing and has a zero gradient, whatever it holds.  A class that stands twice in a row
     counts as two entries.  Gradients reach `predicts` only; logits aliased by join_grads are served like soft_cross_entropy's."""
