@@ -725,3 +725,46 @@ def test_no_starts_make_a_kernel_leave_its_tensors(dtype, Tq, Tk, S, heads, dh, 
             n = lambda c: (c[1:] - c[:-1]).tolist()
             val, tol = definition(q, k, v, dout, at(cu_q), n(cu_q), at(cu_k), n(cu_k), True, dh ** -0.5, 2.0 ** -8 if dtype == BF16 else F)
             check((out, dq, dk, dv), val, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,dh,lq,lk", [
+    ((4, 4), 64, [3, 9, 30], None), ((4, 2), 64, [300, 130], None), ((4, 2), 128, [300, 130], None), ((8, 2), 64, [1, 2], [3000, 1700]),
+    ((2, 2), 64, [40, 30], [500, 300]), ((6, 2), 128, [40, 30], [500, 300]), ((8, 1), 64, [1500], [300])])
+def test_rows_of_small_and_large_scores_side_by_side(dtype, causal, heads, dh, lq, lk):
+    """every row has a size of its own, 2^-6 .. 2^60 (scores exact, as above), so that waves hold rows near and far from zero"""
+    H, Hkv = heads
+    p = problem(dtype, H, Hkv, dh, lq, lk, seed=12)
+    g = torch.Generator().manual_seed(13)
+    q, k = torch.zeros(p["q"].shape), torch.zeros(p["k"].shape)
+    q[..., 5] = 2.0 ** torch.tensor([-6, 0, 4, 9, 11, 20, 60])[torch.randint(0, 7, q.shape[:2], generator=g)]
+    q[..., 5] *= torch.where(torch.rand(q.shape[:2], generator=g) < 0.5, 1.0, -1.0)
+    k[..., 5] = 1 + torch.randint(0, 7, k.shape[:2], generator=g) / 8.0
+    got = [t.double().cpu() for t in run({**p, "q": q.to(dtype).cuda(), "k": k.to(dtype).cuda()}, causal=causal, scale=1.0)]
+    u = 2.0 ** -8 if dtype == BF16 else F
+    Q, K, V, dO = q.double(), k.double(), p["v"].double().cpu(), p["dout"].double().cpu()
+    val, tol = [torch.zeros_like(x) for x in got], [torch.zeros_like(x) for x in got]
+    # p: sums of up to m terms, (m + 16) F; below 2^10 a score times log2 e is rounded by up to 2^-15, four times; rounded to u as an operand
+    rel = (max(p["lk"]) + 16) * F + u + 2.0 ** -13
+    D = 2 * (dO.abs().amax(2).max() * V.abs().sum(2).max())                        # at least |dP| + |delta|
+    count = (H // Hkv) * max(p["lq"]) + 16
+    err = (rel + u + (4 * (dh + 16) + count) * F) * D
+    for a, n, b, m in zip(p["q0"], p["lq"], p["k0"], p["lk"]):
+        seen = torch.ones(n, m, dtype=torch.bool)
+        if causal:
+            seen = torch.arange(m)[None, :] <= torch.arange(n)[:, None] + (m - n)
+        for h in range(H):
+            at, rows, kh = slice(b, b + m), slice(a, a + n), h // (H // Hkv)
+            P = torch.softmax((Q[rows, h, 5][:, None] * K[at, kh, 5]).masked_fill(~seen, -math.inf), 1).nan_to_num(0.0)
+            dP = dO[rows, h] @ V[at, kh].T
+            dS = P * (dP - (dP * P).sum(1, keepdim=True))
+            val[0][rows, h], val[1][rows, h] = P @ V[at, kh], dS @ K[at, kh]
+            val[2][at, kh] += dS.T @ Q[rows, h]
+            val[3][at, kh] += P.T @ dO[rows, h]
+            tol[0][rows, h], tol[1][rows, h] = rel * V.abs().max(), err * 2
+            tol[2][at, kh] += err * (P.T @ Q[rows, h].abs())
+            tol[3][at, kh] += (rel + count * F) * (P.T @ dO[rows, h].abs())
+    for x, w, t, name in zip(got, val, tol, ("O", "dQ", "dK", "dV")):
+        assert ((x - w).abs() <= u * w.abs() + t + 1e-30).all(), name
